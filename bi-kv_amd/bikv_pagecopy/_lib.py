@@ -22,6 +22,7 @@ HINT_NONE, HINT_LAYER_MAJOR, HINT_PAGE_MAJOR = 0, 1, 2
 STAGE_PIPELINED, STAGE_DIRECT, STAGE_AUTO, STAGE_PIPELINED_KERNEL = 0, 1, 2, 3
 TRACE_KINDS = ("kernel", "copy_d2h", "copy_h2d", "copy_kernel")
 PLACE_SPREAD, PLACE_SEQUENTIAL = 0, 1
+T_BF16, T_FP16 = 0, 1
 
 
 class PoolDesc(C.Structure):
@@ -67,6 +68,37 @@ class NHDDesc(C.Structure):
         ("kv_stride_elems", C.c_int64),
         ("token_stride_elems", C.c_int64),
         ("layer_base", C.POINTER(C.c_void_p)),
+    ]
+
+
+class FP8CacheDesc(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32),
+        ("n_layers", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_tokens", C.c_int32),
+        ("reserved", C.c_int32),
+        ("n_pages", C.c_int64),
+        ("page_stride_bytes", C.c_int64),
+        ("token_stride_bytes", C.c_int64),
+        ("scale_page_stride_bytes", C.c_int64),
+        ("plane_base", C.POINTER(C.c_void_p)),
+        ("scale_plane_base", C.POINTER(C.c_void_p)),
+    ]
+
+
+class SeqBatchDesc(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int64),
+        ("max_pages", C.c_int64),
+        ("kv_lens", C.c_void_p),
+        ("q_starts", C.c_void_p),
+        ("n_seqs", C.c_int64),
+        ("n_rows", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -137,6 +169,15 @@ _SIGNATURES = {
                                     C.c_void_p, C.c_int64, C.c_void_p]),
     "bikv_scatter_pages": (C.c_int, [C.c_void_p, C.POINTER(PageBatchDesc), C.c_void_p, C.c_int64,
                                      C.c_void_p, C.c_int64, C.c_void_p]),
+    "bikv_copy_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "bikv_fp8_cache_create": (C.c_int, [C.POINTER(FP8CacheDesc), C.POINTER(C.c_void_p)]),
+    "bikv_fp8_cache_destroy": (C.c_int, [C.c_void_p]),
+    "bikv_fp8_append": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SeqBatchDesc), C.c_void_p, C.c_int64, C.c_int64,
+                                  C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
+    "bikv_fp8_attend_workspace": (C.c_int64, [C.c_void_p, C.POINTER(SeqBatchDesc), C.c_int32]),
+    "bikv_fp8_attend": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SeqBatchDesc), C.c_void_p, C.c_int64, C.c_int64,
+                                  C.c_int32, C.c_int32, C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                  C.c_void_p, C.c_int64, C.c_void_p]),
     "bikv_stager_create": (C.c_int, [C.c_int, C.c_int64, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
     "bikv_stager_wait": (C.c_int, [C.c_void_p, C.POINTER(StageStats)]),
     "bikv_stager_trace": (C.c_int, [C.c_void_p, C.c_int64]),

@@ -264,6 +264,39 @@ class PagedKVPool:
         """staging -> pool on the current stream (asynchronous). Page ids must be unique."""
         self._move(_lib.load().bikv_scatter_pages, batch, staging, scale_staging)
 
+    def page_moves(self, src_ids, dst_ids):
+        """Checks and uploads host lists of page ids for copy_pages, in one upload: returns (src, dst) device tensors.
+        Raises RuntimeError for an id outside the pool, a destination named twice, and a page that is both a source and
+        another entry's destination (the copies of one call are not ordered)."""
+        src = np.ascontiguousarray(np.asarray(src_ids, dtype=np.int64).reshape(-1))
+        dst = np.ascontiguousarray(np.asarray(dst_ids, dtype=np.int64).reshape(-1))
+        if src.size != dst.size:
+            raise RuntimeError("src_ids and dst_ids differ in length")
+        for name, ids in (("src_ids", src), ("dst_ids", dst)):
+            if ids.size and (ids.min() < 0 or ids.max() >= self.n_pages):
+                raise RuntimeError(f"{name} holds a page id outside [0, {self.n_pages})")
+        _lib.require_unique(dst, "copy_pages destination")
+        real = src != dst
+        both = np.intersect1d(src[real], dst[real])
+        if both.size:
+            raise RuntimeError(f"page {int(both[0])} is a source and a destination of one copy: copy in two calls")
+        dev = torch.from_numpy(np.stack([src, dst])).to(self.device)
+        return dev[0], dev[1]
+
+    def copy_pages(self, src_ids: torch.Tensor, dst_ids: torch.Tensor):
+        """Page dst_ids[i] becomes a copy of page src_ids[i], all planes, payload and scales, on the current
+        stream (asynchronous): a fork's partly filled last page, a compaction's moves. Both are int64 device
+        tensors, as page_moves makes them from host lists; ids made on the device must satisfy what
+        it checks (an id outside the pool is skipped and reported by check(), the others are the caller's word)."""
+        for name, t in (("src_ids", src_ids), ("dst_ids", dst_ids)):
+            if t.device != self.device or t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous 1-D int64 tensor on the pool's device")
+        if src_ids.numel() != dst_ids.numel():
+            raise RuntimeError("src_ids and dst_ids differ in length")
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.load().bikv_copy_pages(self._h, src_ids.data_ptr(), dst_ids.data_ptr(), src_ids.numel(),
+                                                   _stream_ptr(self.device)))
+
     def check(self):
         """Synchronises the current stream and raises if a kernel rejected a page id or slot."""
         with torch.cuda.device(self.device):

@@ -1,0 +1,92 @@
+// Internal launch interface between the 8-bit cache's C ABI (fp8_cache_abi.hip) and its gfx950 kernels
+// (fp8_cache_append.hip, fp8_cache_attend.hip). Not installed; the public surface is
+// include/bikv_pagecopy.h.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace bikv {
+
+// n / d for 0 <= n < 2^31 without a division: (n * mul) >> shift with mul = floor(2^shift / d) + 1,
+// shift = 31 + ceil(log2 d). The multiplier is too large by e <= 1 (in units of 2^shift / d), and
+// n * e * d < 2^31 * 2^ceil(log2 d), so the quotient is exact.
+struct FastDiv {
+  uint32_t d;
+  uint32_t shift;
+  uint64_t mul;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return {d, 31 + s, (uint64_t(1) << (31 + s)) / d + 1};
+}
+
+// The sequences of one call: where their pages are, how long they are, which rows of the caller's
+// tensors are theirs. All arrays are device memory.
+struct SeqArgs {
+  const int64_t* table;      // [n_seqs][max_pages], rows table_stride elements apart
+  int64_t table_stride;
+  const int64_t* kv_lens;    // tokens of each sequence, the call's own included
+  const int64_t* q_starts;   // n_seqs + 1 row numbers, or null: sequence b owns row b
+  int64_t n_seqs;
+  int64_t n_rows;            // rows of the caller's tensors
+  int64_t max_len;           // max_pages * page_tokens, below 2^31
+};
+
+// One layer of the cache.
+struct LayerArgs {
+  char* k;                   // payload planes
+  char* v;
+  char* ks;                  // scale planes, fp32
+  char* vs;
+  int64_t n_pages;
+  int64_t page_stride;       // bytes
+  int64_t token_stride;      // bytes
+  int64_t scale_stride;      // bytes between the scales of two pages
+  FastDiv page_tokens;
+  int32_t heads;
+};
+
+struct AppendArgs {
+  SeqArgs seq;
+  LayerArgs layer;
+  const uint16_t* k;         // [n_rows][heads][head_dim]
+  const uint16_t* v;
+  int64_t k_row, k_head, v_row, v_head;   // strides in elements
+  int64_t units;             // page slots of the launch, see the kernel
+  uint32_t* status;
+};
+// type: 0 = bf16, 1 = fp16
+hipError_t launch_fp8_append(int head_dim, int type, const AppendArgs& a, hipStream_t stream);
+
+struct AttendArgs {
+  SeqArgs seq;
+  LayerArgs layer;
+  const uint16_t* q;         // [n_rows][heads * group][head_dim]
+  uint16_t* out;
+  float* lse;                // [n_rows][heads * group], or null
+  int64_t q_row, q_head, o_row, o_head;   // strides in elements
+  FastDiv group;             // query heads to a KV head
+  int32_t causal;
+  float scale_log2;          // softmax scale * log2(e)
+  float* part_o;             // partial results, see the kernels
+  float* part_ml;
+  int32_t slots;             // few rows: shares the work is cut into; many rows: parts a tile's keys are cut into
+  int32_t min_steps;         // few rows: key steps a share has at least
+  int64_t tiles;             // many rows: row tiles of the launch
+  uint32_t* status;
+};
+enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_FEW_64 = 2, ATTEND_MANY = 3 };
+struct AttendPlan {
+  int form;
+  int rows;                  // rows of a tile
+  int32_t slots;
+  int32_t min_steps;
+  int64_t tiles;
+  int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
+};
+// The form a call takes, from what the host knows of it alone.
+AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, int64_t n_rows, int64_t max_len);
+hipError_t launch_fp8_attend(const AttendPlan& plan, int head_dim, int type, const AttendArgs& a, hipStream_t stream);
+
+}  // namespace bikv

@@ -455,6 +455,44 @@ extern "C" int bikv_scatter_pages(const bikv_pool* pool, const bikv_page_batch* 
   return move_pages(ST_BANK_SHARED, 1, pool, batch, staging, staging_bytes, scale_staging, scale_staging_bytes, stream);
 }
 
+extern "C" int bikv_copy_pages(const bikv_pool* pool, const int64_t* src_ids, const int64_t* dst_ids, int64_t n, void* stream) {
+  if (!pool) return fail(BIKV_EINVAL, "null pool");
+  if (n < 0) return fail(BIKV_EINVAL, "negative n");
+  if (n == 0) return BIKV_OK;
+  if (!src_ids || !dst_ids) return fail(BIKV_EINVAL, "src_ids and dst_ids must be non-null");
+  if (n >= (int64_t(1) << 31)) return fail(BIKV_ERANGE, "too many pages for one call");
+  int rc = check_unique_on_device(pool->device, dst_ids, n, static_cast<hipStream_t>(stream));
+  if (rc) return rc;
+  PageMoveArgs a;
+  memset(&a, 0, sizeof(a));
+  rc = device_status(pool->device, ST_BANK_SHARED, &a.status);
+  if (rc) return rc;
+  a.src_ids = src_ids;
+  a.dst_ids = dst_ids;
+  a.n = n;
+  a.n_pool_pages = pool->n_pages;
+  a.n_planes = (uint32_t)pool->n_planes;
+  a.payload.plane_base = pool->d_plane_base;
+  a.payload.tile_bytes = pool->tile_bytes;
+  a.payload.page_stride = pool->page_stride;
+  a.payload.row_bytes = pool->row_bytes;
+  a.payload.row_stride = pool->row_stride;
+  a.payload.log2_row = -1;
+  if ((pool->row_bytes & (pool->row_bytes - 1)) == 0)
+    for (a.payload.log2_row = 0; (int64_t(1) << a.payload.log2_row) < pool->row_bytes;) ++a.payload.log2_row;
+  a.payload.vec_width = lowbit_width(pool->align_bits);
+  if (pool->scale_tile_bytes > 0) {
+    a.scale.plane_base = pool->d_plane_base + pool->n_planes;
+    a.scale.tile_bytes = pool->scale_tile_bytes;
+    a.scale.page_stride = pool->scale_page_stride;
+    a.scale.vec_width = lowbit_width(pool->scale_align_bits);
+  }
+  BIKV_DEVICE(pool->device);
+  const hipError_t e = launch_page_moves(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail_hip(e, "page copy launch");
+  return BIKV_OK;
+}
+
 // The device that owns the memory behind `p`, or -1 when the runtime does not know the pointer or it is
 // host memory.
 static int device_of_pointer(const void* p) {

@@ -104,6 +104,27 @@ hipError_t launch_copy_runs(const RunArgs& a, hipStream_t stream);
 // pinned host memory).
 hipError_t launch_linear_copy(const void* src, void* dst, int64_t bytes, hipStream_t stream);
 
+// Copies inside the pool: page dst_ids[i] becomes a copy of page src_ids[i].
+struct PageMoveClass {
+  const char* const* plane_base;  // device-resident table
+  int64_t tile_bytes, page_stride, row_bytes, row_stride;
+  int32_t log2_row;               // log2(row_bytes) when that is a power of two, else -1
+  int32_t vec_width;              // widest power of two (<= 16) dividing every address and size
+  uint32_t parts;                 // payload: pieces of 64 vectors per tile; scale: vectors per tile
+  uint32_t n_blocks;
+};
+struct PageMoveArgs {
+  PageMoveClass payload;
+  PageMoveClass scale;            // tile_bytes == 0 when the pool has no scale class
+  const int64_t* src_ids;
+  const int64_t* dst_ids;
+  int64_t n;
+  int64_t n_pool_pages;
+  uint32_t n_planes;
+  uint32_t* status;
+};
+hipError_t launch_page_moves(PageMoveArgs& a, hipStream_t stream);
+
 // Fused page move + layout change between token-major pages and a per-layer paged NHD pool.
 struct TransposeArgs {
   const char* const* layer_base;  // device-resident table, n_layers entries

@@ -205,6 +205,14 @@ int bikv_scatter_pages(const bikv_pool* pool, const bikv_page_batch* batch,
                        const void* scale_staging, int64_t scale_staging_bytes,
                        void* stream);
 
+/* copy inside the pool: page dst_ids[i] becomes a copy of page src_ids[i], all planes, payload and scale tiles, for
+ * every i < n. Both arrays are int64 device arrays. This is what a fork of a sequence (its partly filled last page)
+ * and a compaction (pages from the far end into the holes) move. No page may be both a source and another entry's destination, nor a
+ * destination twice (the copies of one launch are not ordered); sources may repeat. An entry with an id outside the
+ * pool is skipped and raises BIKV_ST_PAGE_ID. Asynchronous on stream. The reference's page managers only hand ids out
+ * (DistributedStorage/PageManager.py:20-49); nothing there moves a page inside a pool. */
+int bikv_copy_pages(const bikv_pool* pool, const int64_t* src_ids, const int64_t* dst_ids, int64_t n, void* stream);
+
 /* --------------------------------------------------------------------------------------------
  * 3. Device <-> pinned-host staging pipeline.
  *
@@ -451,6 +459,85 @@ int bikv_nhd_load_token_major(const bikv_nhd* pool, const void* tm, int64_t tm_b
 int bikv_nhd_store_token_major(const bikv_nhd* pool, void* tm, int64_t tm_bytes,
                                const int64_t* block_ids, const int64_t* tm_pages, int64_t n_pages,
                                void* stream);
+
+/* --------------------------------------------------------------------------------------------
+ * 3c. The 8-bit cache: appending to it and attending over it.
+ *
+ * A cache whose K and V are held as e4m3 bytes with one fp32 scale for each (page, head): byte c of a page and
+ * head stands for e4m3(c) * scale. It is the pool of the layered calls above with a scale class (plane 2*layer + kv; a
+ * tile is page_tokens rows of kv_heads * head_dim bytes, a scale tile kv_heads floats), so pages of it are
+ * gathered, scattered, staged and copied by those calls with their scales. The reference holds its cache in fp16 and
+ * attends through a library (Bi-KV/Model/qwen2.py:169-181); this is the same step over the smaller cache.
+ *
+ * Both calls take the sequences of a step as device arrays, so a captured graph can be replayed with other lengths:
+ *   page_table   [n_seqs][max_pages] page ids, rows page_table_stride elements apart; entries behind a sequence's
+ *                last page are not read
+ *   kv_lens      [n_seqs] tokens of each sequence in the cache, the call's own tokens included (append writes
+ *                them, attend is called after it)
+ *   q_starts     [n_seqs + 1] rows q_starts[b] .. q_starts[b+1] of the call's tensors are sequence b's newest tokens, in
+ *                order; NULL = one row per sequence (n_rows == n_seqs). Rows before q_starts[0] and from q_starts[n_seqs] on belong to
+ *                nobody: they are not read, and attend leaves them as they were.
+ * A sequence whose numbers make no sense (a length that is negative or more than its table row holds, rows outside the
+ * tensors, for append more rows than tokens) is skipped as a whole and raises BIKV_ST_SRC_RANGE; a page id outside the pool
+ * raises BIKV_ST_PAGE_ID and its tokens are left out. Asynchronous on `stream`, no allocation, graph-capturable.
+ * Row and head strides are in elements, multiples of 8; addresses are 16-byte aligned; a head's values are contiguous.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct bikv_fp8_cache bikv_fp8_cache; /* opaque; host memory only */
+
+typedef struct bikv_fp8_cache_desc {
+  int32_t device;
+  int32_t n_layers;
+  int32_t kv_heads;
+  int32_t head_dim;                    /* 64 or 128 */
+  int32_t page_tokens;
+  int32_t reserved;
+  int64_t n_pages;
+  int64_t page_stride_bytes;           /* multiple of 16 */
+  int64_t token_stride_bytes;          /* multiple of 16, >= kv_heads * head_dim */
+  int64_t scale_page_stride_bytes;     /* multiple of 4, >= kv_heads * 4 */
+  const void* const* plane_base;       /* HOST array of 2*n_layers device pointers, 16-byte aligned */
+  const void* const* scale_plane_base; /* HOST array of 2*n_layers device pointers to floats */
+} bikv_fp8_cache_desc;
+
+int bikv_fp8_cache_create(const bikv_fp8_cache_desc* desc, bikv_fp8_cache** out);
+int bikv_fp8_cache_destroy(bikv_fp8_cache* cache);
+
+enum { BIKV_T_BF16 = 0, BIKV_T_FP16 = 1 };
+
+typedef struct bikv_seq_batch {
+  const int64_t* page_table;
+  int64_t page_table_stride;
+  int64_t max_pages;
+  const int64_t* kv_lens;
+  const int64_t* q_starts;
+  int64_t n_seqs;
+  int64_t n_rows;
+  int32_t dtype;                       /* BIKV_T_*: type of the call's tensors */
+  int32_t reserved;
+} bikv_seq_batch;
+
+/* k, v: [n_rows][kv_heads][head_dim]. Per (page, head), K and V apart, over the finite new values of the page:
+ *   need = the smallest power of two >= 2^-126 with max|x| <= 448 need
+ *   scale = need where the page holds no older token of the sequence; else the old scale while 448 scale >= max|x|, and
+ *           need otherwise, the older tokens' bytes being rounded once more to the new scale
+ *   byte = e4m3(x / scale), nearest, ties to even; NaN and infinities become NaN.
+ * Positions behind the new tokens are left as they were. A page may be the target of one sequence of a call only. */
+int bikv_fp8_append(const bikv_fp8_cache* cache, int32_t layer, const bikv_seq_batch* batch,
+                    const void* k, int64_t k_row_stride, int64_t k_head_stride,
+                    const void* v, int64_t v_row_stride, int64_t v_head_stride, void* stream);
+
+/* q, out: [n_rows][q_heads][head_dim]; q_heads a multiple of kv_heads (query head i reads KV head
+ * i / (q_heads / kv_heads)). Row t of a sequence with n rows sees all of its kv_len keys or, causal, the first
+ * kv_len - n + t + 1. out = softmax(softmax_scale q.K) V; lse (nullable, [n_rows][q_heads] floats, contiguous) is the natural
+ * logarithm of the softmax's sum. A row that sees no key gets out = 0, lse = -inf. Whatever lies in keys a row does
+ * not see, NaN included, does not reach it. `workspace`: device memory of bikv_fp8_attend_workspace() bytes (0 = none
+ * needed) that belongs to this call until it has run: calls that may overlap take one each. out must not overlap q. */
+int64_t bikv_fp8_attend_workspace(const bikv_fp8_cache* cache, const bikv_seq_batch* batch, int32_t q_heads);
+int bikv_fp8_attend(const bikv_fp8_cache* cache, int32_t layer, const bikv_seq_batch* batch,
+                    const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t q_heads,
+                    int32_t causal, float softmax_scale,
+                    void* out, int64_t out_row_stride, int64_t out_head_stride, float* lse,
+                    void* workspace, int64_t workspace_bytes, void* stream);
 
 /* --------------------------------------------------------------------------------------------
  * 4. Producer/consumer ring — the `ipc_service` roles.
