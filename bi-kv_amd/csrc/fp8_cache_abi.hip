@@ -152,9 +152,15 @@ static int plan_call(const bikv_fp8_cache* c, const bikv_seq_batch* b, int32_t q
   *plan = AttendPlan();
   if (b->n_seqs == 0 || b->n_rows == 0) return BIKV_OK;
   *plan = plan_fp8_attend(c->head_dim, c->heads, q_heads / c->heads, b->n_seqs, b->n_rows, b->max_pages * c->page_tokens);
-  if (plan->form == ATTEND_MANY && plan->tiles * c->heads * plan->slots * 32 >= (int64_t(1) << 31))
+  if (plan->tiles * c->heads * (plan->form == ATTEND_MANY ? plan->slots * 32 : 1) >= (int64_t(1) << 31))
     return fail(BIKV_ERANGE, "too many rows times heads for one call");
   return BIKV_OK;
+}
+
+// Parts' results, their (m, l), and the slots' words on joining them; part_rows is even, so the last are 8-byte aligned.
+static int64_t workspace_bytes_of(const bikv_fp8_cache* c, const AttendPlan& p) {
+  if (p.part_rows == 0) return 0;
+  return p.part_rows * (c->head_dim + 2) * 4 + (p.form == ATTEND_MANY ? 0 : p.slots * (int64_t)sizeof(JoinHead));
 }
 
 }  // namespace bikv
@@ -163,7 +169,7 @@ extern "C" int64_t bikv_fp8_attend_workspace(const bikv_fp8_cache* c, const bikv
   AttendPlan p;
   const int rc = plan_call(c, b, q_heads, &p);
   if (rc) return rc;
-  return p.part_rows * (c->head_dim + 2) * 4;
+  return workspace_bytes_of(c, p);
 }
 
 extern "C" int bikv_fp8_attend(const bikv_fp8_cache* c, int32_t layer, const bikv_seq_batch* b, const void* q, int64_t q_row_stride,
@@ -181,7 +187,7 @@ extern "C" int bikv_fp8_attend(const bikv_fp8_cache* c, int32_t layer, const bik
   if (!rc) rc = check_rows("out", out, out_row_stride, out_head_stride);
   if (rc) return rc;
   if ((uintptr_t)lse % 4 != 0) return fail(BIKV_EINVAL, "lse must be 4-byte aligned");
-  const int64_t need = p.part_rows * (c->head_dim + 2) * 4;
+  const int64_t need = workspace_bytes_of(c, p);
   if (need > 0 && (!workspace || (uintptr_t)workspace % 16 != 0 || workspace_bytes < need))
     return fail(BIKV_EINVAL, "workspace must be 16-byte aligned and hold %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
   if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0.f) return fail(BIKV_EINVAL, "softmax_scale must be finite");
@@ -197,6 +203,7 @@ extern "C" int bikv_fp8_attend(const bikv_fp8_cache* c, int32_t layer, const bik
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + p.part_rows * c->head_dim;
+  a.part_join = reinterpret_cast<JoinHead*>(a.part_ml + 2 * p.part_rows);
   rc = device_status(c->device, ST_BANK_SHARED, &a.status);
   if (rc) return rc;
   BIKV_DEVICE(c->device);

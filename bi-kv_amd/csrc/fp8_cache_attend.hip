@@ -48,6 +48,7 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
 }
+__device__ __forceinline__ float half_of(uint32_t pair, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> (16 * i))); }
 template <int TYPE>
 __device__ __forceinline__ uint32_t narrow(float a, float b) {
   if constexpr (TYPE == 0)
@@ -56,10 +57,19 @@ __device__ __forceinline__ uint32_t narrow(float a, float b) {
     return pack_f16(a, b);
 }
 
-// 0xffff in each half that is a NaN in fp16.
-__device__ __forceinline__ uint32_t nan_halves(uint32_t x) {
-  const uint32_t t = ((x & 0x7fff7fffu) + 0x03ff03ffu) & 0x80008000u;    // sign bit set where the magnitude is over 0x7c00
-  return (t >> 15) * 0xffffu;
+// 0xff in each byte that is a NaN in e4m3.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
+// Reads one key's row of V again and keeps, by place, the first key that holds a NaN there. Rows see keys up to some
+// position, so a row's output is NaN at a place exactly if that first key is one it sees. Rare: small, not fast.
+template <int D>
+__device__ __forceinline__ void note_nans(int* nan_at, uint64_t row, int pos) {
+#pragma nounroll
+  for (int d = 0; d < D; d += 4) {
+    uint32_t bad = nan_bytes(gload<uint32_t>(row + d));
+#pragma nounroll
+    for (int k = 0; bad != 0; ++k, bad >>= 8)
+      if (bad & 1u) atomicMin(nan_at + d + k, pos);
+  }
 }
 
 // Exponent of a page's V scale, -126 where it is zero, subnormal or not finite.
@@ -71,141 +81,243 @@ __device__ __forceinline__ int scale_exponent(float s) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---------------------------------------------------------------------------------------------
-// Few rows per sequence: one wave per (tile of up to 64 rows, KV head, run of key steps).
+// Few rows per sequence: a workgroup takes a tile of 16, 32 or 64 rows over a run of key steps, its waves the KV
+// heads; where there are more waves than heads, several waves share a head and take its steps in turn.
 //
-// Bound by memory: every byte of K and V is read once per row tile. Waves share nothing and never meet at a
-// barrier. A lane reads its operands' bytes straight from the cache: for K 16 bytes of a
-// key's row (a matrix product does not mind in which order it sums, so the four lanes of a row take the
-// 16-byte pieces as they lie), for V the D/16 bytes at one place of its own eight keys' rows, which the
-// lane transposes in registers. The loads of the next step are issued before the present one is computed.
+// Bound by memory: every byte of K and V is read once per row tile. Each wave copies its own steps' rows into its own part
+// of LDS (global_load_lds, 16 bytes a lane, whole rows) and never waits for another wave while it goes: scales and the next
+// page ids first, then K, then V, each refilled for the next step as soon as it has been read, with the waits
+// counted by hand. The heads of a page stand side by side in memory, so the waves of a workgroup together read whole
+// pages: copies alone run at 6.2 TB/s this way and at 5.2 TB/s with every head in a workgroup of its own. From LDS a lane takes its
+// operands' bytes: for K 16 bytes of a key's row (a matrix product does not mind in which order it sums, so the four lanes
+// of a row take the 16-byte pieces as they lie), for V the D/16 bytes at one place of its own eight keys' rows, which it
+// transposes in registers. At the end the waves of a head join their sums in LDS.
 //
-// The work is cut evenly: row tiles of all sequences times their key steps form one line, share s of
-// it belongs to slot s (every KV head has its own wave per slot). A tile that lies in one share is
-// finished there; the others leave (O, m, l) per share and fp8_join_few_kernel joins them.
+// Two ways of cutting the work, chosen by the host: every tile a workgroup of its own (no second launch), or, where sequences
+// may be long, even shares: the tiles of all sequences times their key steps form one line, share s of which is slot s's.
+// A tile that lies in one share is finished there; of the others each share leaves (O, m, l), and
+// fp8_join_few_kernel joins them.
 // ---------------------------------------------------------------------------------------------
 template <int D, int TYPE, int NT, int NK>
 struct Few {
   static constexpr int kM = 16 * NT;       // rows of a tile
+  static constexpr int kWaves = NT <= 2 ? 8 : 4;   // 8 waves of 256 registers fill a CU, 4 of 512
   static constexpr int kKeys = 16 * NK;    // keys of a step
   static constexpr int kDT = D / 16;       // bytes of a V row per lane, and row tiles of O^T
+  static constexpr int kChunks = D / 16;   // 16-byte pieces of a key's row
+  static constexpr int kCopies = kKeys * D / 1024;   // copies of 1 KiB that bring a step's K (or V)
 };
 
-__device__ __forceinline__ int64_t tiles_of(const Seq& s, const FastDiv& group, int m) {
-  return ((int64_t)s.n * group.d + m - 1) / m;
+// Global memory straight into LDS: lane i's 16 (4) bytes land at `lds` + 16 i (4 i). Written out so that the kernel
+// itself says which copies it waits for: the compiler would wait for all of them before any read of LDS.
+__device__ __forceinline__ void copy16_to_lds(uint64_t src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
 }
-__device__ __forceinline__ int steps_of(const Seq& s, int keys) { return s.len <= keys ? 1 : (s.len + keys - 1) / keys; }
-
-// The line of work, as one wave sees it.
-struct Line {
-  int64_t total;    // steps
-  int64_t begin;    // of this share
-  int64_t end;
-};
-__device__ __forceinline__ Line share_of(int64_t total, int slots, int min_steps, int slot) {
-  const int64_t want = (total + min_steps - 1) / min_steps;
-  const int64_t n = want < slots ? (want > 0 ? want : 1) : slots;
-  const int64_t per = total / n, more = total - per * n;
-  Line l;
-  l.total = total;
-  l.begin = slot < n ? slot * per + (slot < more ? slot : more) : total;
-  l.end = slot < n ? l.begin + per + (slot < more ? 1 : 0) : total;
-  return l;
+__device__ __forceinline__ void copy4_to_lds(uint64_t src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory");
 }
-// The share that step x of the line lies in.
-__device__ __forceinline__ int slot_of(int64_t total, int slots, int min_steps, int64_t x) {
-  const int64_t want = (total + min_steps - 1) / min_steps;
-  const int64_t n = want < slots ? (want > 0 ? want : 1) : slots;
-  const int64_t per = total / n, more = total - per * n;
-  const int64_t cut = more * (per + 1);
-  return (int)(x < cut ? x / (per + 1) : more + (x - cut) / per);
+// Waits until at most N of the wave's newest vector memory accesses are under way.
+template <int N>
+__device__ __forceinline__ void wait_vmem() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+// A barrier for what the workgroup has in LDS: __syncthreads would also wait until stores to global memory have arrived.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+template <class T>
+__device__ __forceinline__ uint32_t lds_address(T* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)p;
 }
 
+__device__ __forceinline__ uint32_t tiles_of(const Seq& s, const FastDiv& group, int m) { return ((uint32_t)s.n * group.d + m - 1) / m; }
+__device__ __forceinline__ uint32_t steps_of(const Seq& s, int keys) { return s.len <= keys ? 1 : ((uint32_t)s.len + keys - 1) / keys; }
 template <int M, int KEYS>
-__device__ __forceinline__ int64_t line_length(const AttendArgs& a, int lane) {
-  int64_t sum = 0;
-  for (int64_t b = lane; b < a.seq.n_seqs; b += 64) {
-    const Seq s = read_seq(a.seq, b);
-    sum += tiles_of(s, a.group, M) * steps_of(s, KEYS);
+__device__ __forceinline__ uint32_t weight_of(const AttendArgs& a, int64_t b) {
+  if (b >= a.seq.n_seqs) return 0;
+  const Seq s = read_seq(a.seq, b);
+  if (!s.ok) raise_flag(a.status, ST_SLOT_SRC);
+  return tiles_of(s, a.group, M) * steps_of(s, KEYS);
+}
+
+// The number of the row tile that sequence b's first row begins, if every sequence may leave one tile unfilled: a rising
+// function of b with room for all of its tiles.
+template <int M>
+__device__ __forceinline__ int64_t first_tile(const AttendArgs& a, int64_t b) {
+  int64_t q = b;
+  if (a.seq.q_starts) {
+    q = a.seq.q_starts[b];
+    q = q < 0 ? 0 : q > a.seq.n_rows ? a.seq.n_rows : q;
   }
-  return uni64(wave_sum64(sum));
+  return q * a.group.d / M + b;
+}
+
+// The line's length (the host sees to it that it stays below 2^31).
+template <int M, int KEYS>
+__device__ __forceinline__ uint32_t line_length(const AttendArgs& a, int lane) {
+  uint32_t sum = 0;
+  for (int64_t b = lane; b < a.seq.n_seqs; b += 64) sum += weight_of<M, KEYS>(a, b);
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+  return (uint32_t)uni((int)sum);
 }
 // The sequence that step x (below the line's length) belongs to, and where in it.
 template <int M, int KEYS>
-__device__ __forceinline__ int64_t seq_at(const AttendArgs& a, int64_t x, int lane, int64_t* local) {
-  int64_t run = 0;
+__device__ __forceinline__ int64_t seq_at(const AttendArgs& a, uint32_t x, int lane, uint32_t* local) {
+  uint32_t run = 0;
   for (int64_t base = 0; base < a.seq.n_seqs; base += 64) {
-    int64_t w = 0;
-    if (base + lane < a.seq.n_seqs) {
-      const Seq s = read_seq(a.seq, base + lane);
-      w = tiles_of(s, a.group, M) * steps_of(s, KEYS);
+    const uint32_t w = weight_of<M, KEYS>(a, base + lane);
+    uint32_t upto = w;
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint32_t y = __shfl_up(upto, m);
+      if (lane >= m) upto += y;
     }
-    const int64_t upto = run + wave_scan64(w, lane);
+    upto += run;
     const uint64_t m = __ballot(upto > x);
     if (m) {
       const int src = __builtin_ctzll(m);
-      *local = uni64(x - shfl64(upto - w, src));
-      return uni64(base + src);
+      *local = (uint32_t)uni((int)(x - __shfl(upto - w, src)));
+      return base + src;
     }
-    run = uni64(shfl64(upto, 63));
+    run = (uint32_t)uni((int)__shfl(upto, 63));
   }
   *local = 0;
   return a.seq.n_seqs;
 }
 
 template <int D, int TYPE, int NT, int NK>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(const AttendArgs a) {
+__global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), (NT <= 2 ? 2 : 1)) void fp8_attend_few_kernel(const AttendArgs a) {
   using C = Few<D, TYPE, NT, NK>;
-  constexpr int kM = C::kM, kKeys = C::kKeys, kDT = C::kDT;
+  constexpr int kM = C::kM, kKeys = C::kKeys, kDT = C::kDT, kChunks = C::kChunks, kCopies = C::kCopies, kWaves = C::kWaves;
   constexpr int kQK = D / 32;              // matrix steps of q . k
   struct Meta {
-    uint64_t off[kKeys];                   // byte offset of the key's row in its plane
+    u32x4 kv[2][kKeys * kChunks];          // K, V
+    uint64_t off[2][kKeys];                // byte offset of the key's row in its plane; of this step and the next
+    float ks_in[64], vs_in[64];            // the copies' targets: a step's scales, the next step's page ids
+    uint32_t pid_in[2][64];
     float ks[kKeys], vs[kKeys];
     int pos[kKeys];
+    int nan_at[D];                         // by place: the first key with a NaN in V that not every row sees
   };
-  __shared__ Meta metas[4];
-  const int wave = uni(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  __shared__ Meta metas[kWaves];
+  __shared__ float sums[kWaves][2][kM];    // the waves' m and l
+  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63;
   const int quad = lane >> 4, col = lane & 15;
   Meta& meta = metas[wave];
-  const uint32_t w = blockIdx.x * 4 + wave;
   const uint32_t H = (uint32_t)a.layer.heads;
-  const int h = (int)(w % H), slot = (int)(w / H);
-  if (slot >= a.slots) return;
+  // the workgroup's heads: `hw` of them from h0 on; wave i does head h0 + i % hw and is its turn i / hw of `ways`
+  const uint32_t hw = (uint32_t)a.heads_per_group, groups = (H + hw - 1) / hw;
+  const int slot = (int)(blockIdx.x / groups), h0 = (int)((blockIdx.x - slot * groups) * hw);
+  const int ways = kWaves / (int)hw, way = wave / (int)hw;
+  const int h_raw = h0 + wave - way * (int)hw;
+  const bool works = way < ways && h_raw < (int)H;
+  const int h = h_raw < (int)H ? h_raw : h0;
   const int G = (int)a.group.d;
   const int P = (int)a.layer.page_tokens.d;
 
-  const int64_t total = line_length<kM, kKeys>(a, lane);
-  if (w == 0)
-    for (int64_t b = lane; b < a.seq.n_seqs; b += 64)
-      if (!read_seq(a.seq, b).ok) raise_flag(a.status, ST_SLOT_SRC);
-  const Line line = share_of(total, a.slots, a.min_steps, slot);
-  if (line.begin >= line.end) return;
-  int64_t local = 0;
-  int64_t b = seq_at<kM, kKeys>(a, line.begin, lane, &local);
-
   const uint64_t kbase = (uint64_t)a.layer.k + h * D, vbase = (uint64_t)a.layer.v + h * D;
   const uint64_t ksbase = (uint64_t)a.layer.ks + 4 * h, vsbase = (uint64_t)a.layer.vs + 4 * h;
+  const uint32_t lds_k = (uint32_t)uni((int)lds_address(meta.kv[0])), lds_v = (uint32_t)uni((int)lds_address(meta.kv[1]));
+  const uint32_t lds_ks = (uint32_t)uni((int)lds_address(meta.ks_in)), lds_vs = (uint32_t)uni((int)lds_address(meta.vs_in));
+  const uint32_t lds_pid = (uint32_t)uni((int)lds_address(meta.pid_in));
+  // rows whose pieces would meet in a bank: those a whole sweep of the 64 banks (256 bytes) apart
+  auto swizzle = [](int row) { return (row / (16 / kChunks)) & (kChunks - 1); };
 
-  int64_t at = line.begin;
+  Seq seq = {0, 0, 0, false};
+  int64_t seq_of = -1;                     // the sequence that `seq` is
+  Share line = {1, 0, 0};
+  JoinHead join = {0, 0, 0, 0, 0};
+  uint32_t local = 0;                      // step of the line within sequence b
+  int64_t b = 0;
+  if (a.slots > 0) {
+    const uint32_t total = line_length<kM, kKeys>(a, lane);
+    line = share_of(total, (uint32_t)a.slots, (uint32_t)a.min_steps, (uint32_t)slot);
+    if (line.begin < line.end) b = seq_at<kM, kKeys>(a, line.begin, lane, &local);
+  } else {
+    b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile<kM>(a, i); });
+    if (h0 == 0 && tid == 0 && slot < a.seq.n_seqs && !read_seq(a.seq, slot).ok) raise_flag(a.status, ST_SLOT_SRC);
+    seq = read_seq(a.seq, b);
+    seq_of = b;
+    const int64_t tile = slot - first_tile<kM>(a, b);
+    if (!seq.ok || tile < 0 || tile >= (int64_t)tiles_of(seq, a.group, kM)) return;
+    const uint32_t steps = (uint32_t)uni((int)steps_of(seq, kKeys));
+    local = (uint32_t)uni((int)tile) * steps;
+    line = {steps, 0, steps};
+  }
+
+  uint32_t at = line.begin;
   while (at < line.end && b < a.seq.n_seqs) {
-    const Seq seq = read_seq(a.seq, b);
-    const int steps = uni(steps_of(seq, kKeys));
-    const int64_t weight = uni64(tiles_of(seq, a.group, kM) * steps);
+    if (seq_of != b) {
+      seq = read_seq(a.seq, b);
+      seq_of = b;
+    }
+    const int steps = uni((int)steps_of(seq, kKeys));
+    const uint32_t weight = (uint32_t)uni((int)(tiles_of(seq, a.group, kM) * (uint32_t)steps));
     if (local >= weight) {
       ++b;
       local = 0;
       continue;
     }
-    const int tile = (int)(local / steps);
-    const int step0 = (int)(local - (int64_t)tile * steps);
+    const int tile = (int)(local / (uint32_t)steps);
+    const int step0 = (int)local - tile * steps;
     int count = steps - step0;
-    if (count > line.end - at) count = (int)(line.end - at);
+    if ((uint32_t)count > line.end - at) count = (int)(line.end - at);
     const bool first_of_share = at == line.begin;
     const bool whole = count == steps;
     const int rows = uni((int)((int64_t)seq.n * G - (int64_t)tile * kM < kM ? (int64_t)seq.n * G - (int64_t)tile * kM : kM));
     const int len = uni(seq.len);
     const int before = a.causal ? uni(seq.len - seq.n) : 0;     // keys older than the call's own (negative: some rows see none)
+    if (step0 == 0 && !whole)
+      join = {seq.first, tile, rows, (int)((at + steps - 1) / line.per) - slot + 1, 2 * slot + (first_of_share ? 0 : 1)};
 
+    const int last_tok = uni((int)divide((uint32_t)(tile * kM + rows - 1), a.group));
+    const int first_tok = uni((int)divide((uint32_t)(tile * kM), a.group));
+    int seen = a.causal ? before + last_tok + 1 : len;           // keys that the tile's last row sees
+    seen = seen < 0 ? 0 : seen;
+    int all = a.causal ? before + first_tok + 1 : len;           // keys that every row sees
+    all = all < 0 ? 0 : all;
+    int end = step0 + count;
+    if (end > (seen + kKeys - 1) / kKeys) end = (seen + kKeys - 1) / kKeys;
+    const int begin = works ? step0 + way : end;                 // the wave's steps: begin, begin + ways, ...
+
+    // A step's copies into LDS, in the order in which they are waited for: scales and the next step's page ids, K, V.
+    // Keys that are not there (behind the sequence, or on a page the pool does not have) read the
+    // plane's first row and are masked by position.
+    const uint64_t trow = (uint64_t)(a.seq.table + b * a.seq.table_stride);
+    auto key_of = [&](int step) { return step * kKeys + (lane & (kKeys - 1)); };
+    auto copy_pages = [&](int step) {
+      int key = key_of(step);
+      key = key < seen ? key : seen - 1;
+      const uint64_t src = trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens);
+      copy4_to_lds(src, lds_pid);
+      copy4_to_lds(src + 4, lds_pid + 256);
+    };
+    bool bad_page = false;
+    auto copy_scales = [&](int step, int which) {                // returns the position of the lane's key
+      const int key = key_of(step);
+      const uint64_t pid = meta.pid_in[0][lane] | ((uint64_t)meta.pid_in[1][lane] << 32);
+      const bool in = key < seen, ok = in && pid < (uint64_t)a.layer.n_pages;
+      bad_page |= in && !ok;
+      const int64_t page = ok ? (int64_t)pid : 0;
+      uint32_t in_page = (uint32_t)key - divide((uint32_t)key, a.layer.page_tokens) * (uint32_t)P;
+      in_page = ok ? in_page : 0;
+      meta.off[which][lane & (kKeys - 1)] = (uint64_t)(page * a.layer.page_stride) + (uint64_t)in_page * (uint64_t)a.layer.token_stride;
+      copy4_to_lds(ksbase + (uint64_t)(page * a.layer.scale_stride), lds_ks);
+      copy4_to_lds(vsbase + (uint64_t)(page * a.layer.scale_stride), lds_vs);
+      return ok ? key : kNoKey;
+    };
+    // A row's 16-byte pieces are XOR-ed with its number on the way, so that reads of a column spread over the banks; a
+    // copy still takes whole rows.
+    auto copy_rows = [&](int which, uint64_t base, uint32_t lds) {       // a loop: its code, not its time, is what the first step waits for
+#pragma nounroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int row = i * (64 / kChunks) + lane / kChunks;
+        copy16_to_lds(base + meta.off[which][row] + 16 * ((lane & (kChunks - 1)) ^ swizzle(row)), lds + 1024 * i);
+      }
+    };
+
+    if (begin < end) copy_pages(begin);
     // The lane's rows: row tile*kM + 16 t + col.
     uint32_t tok[NT];
     int head[NT], limit[NT];
@@ -228,18 +340,17 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(co
         q[t][j + 1] = gload<u32x4>(p + 16);
       }
     }
-    const int last_tok = uni((int)divide((uint32_t)(tile * kM + rows - 1), a.group));
-    const int first_tok = uni((int)divide((uint32_t)(tile * kM), a.group));
-    int seen = a.causal ? before + last_tok + 1 : len;           // keys that the tile's last row sees
-    seen = seen < 0 ? 0 : seen;
-    int all = a.causal ? before + first_tok + 1 : len;           // keys that every row sees
-    all = all < 0 ? 0 : all;
-    int end = step0 + count;
-    if (end > (seen + kKeys - 1) / kKeys) end = (seen + kKeys - 1) / kKeys;
+
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < kQK; ++j) asm volatile("" : "+v"(q[t][j]));     // here before the copies are counted
 
     f32x4 o[NT][kDT];
     float m[NT], l[NT];
     int r_exp = -126;
+    bool spoilt = false;
+    for (int d = lane; d < D; d += 64) meta.nan_at[d] = kNoKey;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kMinusInf;
@@ -248,64 +359,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(co
       for (int i = 0; i < kDT; ++i) o[t][i] = f32x4{0, 0, 0, 0};
     }
 
-    const uint64_t trow = (uint64_t)(a.seq.table + b * a.seq.table_stride);
-    auto page_of = [&](int step) -> int64_t {                   // the page id of the lane's key
-      const int key = step * kKeys + lane;
-      if (lane >= kKeys || key >= seen) return -1;
-      return gload<int64_t>(trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens));
-    };
-    struct Data {
-      u32x4 k[NK][D / 64];
-      uint32_t v[NK][4][kDT / 4];
-      float ks, vs;
-      int pos;
-    };
-    // Issues a step's loads: the page ids are there. Keys that are not there (behind the sequence, or
-    // on a page the pool does not have) read the plane's first row instead, and are masked by position.
-    auto fetch = [&](int step, int64_t pid, Data& x) {
-      const int key = step * kKeys + lane;
-      bool ok = lane < kKeys && key < seen;
-      if (ok && (uint64_t)pid >= (uint64_t)a.layer.n_pages) {
-        raise_flag(a.status, ST_SLOT_PAGE);
-        ok = false;
-      }
-      x.pos = ok ? key : kNoKey;
-      x.ks = 0.f;
-      x.vs = 0.f;
-      uint64_t off = 0;
-      if (ok) {
-        const uint32_t in_page = (uint32_t)key - divide((uint32_t)key, a.layer.page_tokens) * (uint32_t)P;
-        off = (uint64_t)(pid * a.layer.page_stride) + (uint64_t)in_page * (uint64_t)a.layer.token_stride;
-        x.ks = gload<float>(ksbase + (uint64_t)(pid * a.layer.scale_stride));
-        x.vs = gload<float>(vsbase + (uint64_t)(pid * a.layer.scale_stride));
-      }
-      if (lane < kKeys) meta.off[lane] = off;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const uint64_t p = kbase + meta.off[16 * i + col] + 16 * quad;
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) x.k[i][j] = gload<u32x4>(p + 64 * j);
-      }
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint64_t p = vbase + meta.off[16 * i + 4 * quad + e] + kDT * col;
-          if constexpr (kDT == 8) {
-            const u32x2 c = gload<u32x2>(p);
-            x.v[i][e][0] = c[0];
-            x.v[i][e][1] = c[1];
-          } else {
-            x.v[i][e][0] = gload<uint32_t>(p);
-          }
-        }
-    };
-    auto compute = [&](int step, Data& x) {
+    auto compute = [&](int step, int which, int pos, bool more) {
+      wait_vmem<kCopies>();                                      // all but V
+      const float ks_in = meta.ks_in[lane], vs_in = meta.vs_in[lane];
       // a larger V scale than any before: what is summed moves to its exponent
-      const int e = scale_exponent(x.vs);
-      if (__ballot(x.pos != kNoKey && e > r_exp)) {
-        int top = x.pos != kNoKey ? e : -126;
+      const int e = pos != kNoKey ? scale_exponent(vs_in) : -126;
+      if (__ballot(e > r_exp)) {
+        int top = e;
         for (int k = 32; k > 0; k >>= 1) {
           const int y = __shfl_xor(top, k);
           top = y > top ? y : top;
@@ -319,14 +379,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(co
             for (int c = 0; c < 4; ++c) o[t][i][c] = ldexpf(o[t][i][c], r_exp - top);
         r_exp = top;
       }
-      if (lane < kKeys) {
-        meta.ks[lane] = x.ks * a.scale_log2;
-        meta.vs[lane] = ldexpf(x.vs, kPShift - r_exp);
-        meta.pos[lane] = x.pos;
-      }
+      meta.ks[lane & (kKeys - 1)] = ks_in * a.scale_log2;
+      meta.vs[lane & (kKeys - 1)] = ldexpf(vs_in, kPShift - r_exp);
+      meta.pos[lane & (kKeys - 1)] = pos;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const bool edge = (step + 1) * kKeys > all || __ballot(lane < kKeys && x.pos == kNoKey) != 0;
+      const bool edge = (step + 1) * kKeys > all || __ballot(pos == kNoKey) != 0;
 
+      __builtin_amdgcn_sched_barrier(0);
       // S^T = K Q^T
       f32x4 s[NT][NK];
 #pragma unroll
@@ -336,9 +395,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(co
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
           u32x4 f[2];
+          const u32x4 x = meta.kv[0][(16 * i + col) * kChunks + ((4 * j + quad) ^ swizzle(16 * i + col))];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const u32x2 lo = widen4<TYPE>(x.k[i][j][2 * half]), hi = widen4<TYPE>(x.k[i][j][2 * half + 1]);
+            const u32x2 lo = widen4<TYPE>(x[2 * half]), hi = widen4<TYPE>(x[2 * half + 1]);
             f[half] = u32x4{lo[0], lo[1], hi[0], hi[1]};
           }
 #pragma unroll
@@ -348,171 +408,283 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void fp8_attend_few_kernel(co
           }
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      int next = kNoKey;
+      if (more) {
+        next = copy_scales(step + ways, which ^ 1);
+        copy_pages(step + 2 * ways);
+        copy_rows(which ^ 1, kbase, lds_k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       // softmax: the lane's keys are 16 i + 4 quad + c
+      u32x4 p[NT][NK / 2], p_low[NT][TYPE == 1 ? NK / 2 : 1];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        uint32_t hidden = 0;                     // bit per key of the lane: the row does not see it
         float top = kMinusInf;
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
           const f32x4 ks = *reinterpret_cast<const f32x4*>(&meta.ks[16 * i + 4 * quad]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            s[t][i][c] *= ks[c];
-            if (edge && meta.pos[16 * i + 4 * quad + c] >= limit[t]) s[t][i][c] = kMinusInf;
-            top = fmaxf(top, s[t][i][c]);
-          }
+          for (int c = 0; c < 4; ++c) s[t][i][c] *= ks[c];
         }
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (meta.pos[16 * i + 4 * quad + c] >= limit[t]) {
+                s[t][i][c] = kMinusInf;
+                hidden |= 1u << (4 * i + c);
+              }
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) top = fmaxf(top, s[t][i][c]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float now = fmaxf(m[t], top);
-        const float from = now == kMinusInf ? 0.f : now;
-        const float grow = exp2_fast(m[t] - from);              // 0 at the first key
-        m[t] = now;
-        float sum = 0.f;
+        if (__ballot(top > m[t])) {
+          const float now = fmaxf(m[t], top);
+          const float grow = now == kMinusInf ? 1.f : exp2_fast(m[t] - now);       // 0 at the first key
+          m[t] = now;
+          l[t] *= grow;
+#pragma unroll
+          for (int i = 0; i < kDT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[t][i][c] *= grow;
+        }
+        const float from = m[t] == kMinusInf ? 0.f : m[t];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(&meta.vs[16 * i + 4 * quad]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float e = exp2_fast(s[t][i][c] - from);
+            l[t] += e;
+            s[t][i][c] = e * vs[c];
+          }
+        }
+        if (edge) {                              // 0 times a scale that is not finite
+#pragma unroll
+          for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if ((hidden >> (4 * i + c)) & 1u) s[t][i][c] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float f0 = s[t][i][2 * c], f1 = s[t][i][2 * c + 1];
+            const uint32_t y = pack_f16(f0, f1);
+            p[t][i / 2][2 * (i & 1) + c] = y;
+            if constexpr (TYPE == 1) p_low[t][i / 2][2 * (i & 1) + c] = pack_f16(f0 - half_of(y, 0), f1 - half_of(y, 1));
+          }
+      }
+      if (more) wait_vmem<4 + kCopies>();                        // all but what has just been asked for
+      else wait_vmem<0>();
+      uint32_t xv[NK][4][kDT / 4];
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int row = 16 * i + 4 * quad + c;
+          const uint32_t* piece = reinterpret_cast<const uint32_t*>(&meta.kv[1][row * kChunks + ((col * kDT / 16) ^ swizzle(row))]) + (col * kDT / 4) % 4;
+          if constexpr (kDT == 8) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(piece);
+            xv[i][c][0] = x[0];
+            xv[i][c][1] = x[1];
+          } else {
+            xv[i][c][0] = piece[0];
+          }
+        }
+      // V^T operands: eight keys' bytes at four places, transposed
+      auto operands = [&](int i, int dw, u32x4 (&f)[4]) {
+        u32x2 x8[8];                             // [key] -> places (0, 1) and (2, 3) of the dword
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x8[c] = widen4<1>(xv[i + c / 4][c & 3][dw]);
+#pragma unroll
+        for (int pl = 0; pl < 4; ++pl)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            f[pl][c] = __builtin_amdgcn_perm(x8[2 * c + 1][pl / 2], x8[2 * c][pl / 2], pl & 1 ? 0x07060302u : 0x05040100u);
+      };
+      if (edge) {
+        // Bytes of keys that nobody sees become zero, and so does a NaN: the rows that see its key get it at the end.
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[t][i][c] = exp2_fast(s[t][i][c] - from);
-            sum += s[t][i][c];
+            const bool gone = meta.pos[16 * i + 4 * quad + c] == kNoKey;
+#pragma unroll
+            for (int dw = 0; dw < kDT / 4; ++dw) {
+              const uint32_t bytes = gone ? 0 : xv[i][c][dw], bad = nan_bytes(bytes);
+              any |= bad;
+              xv[i][c][dw] = bytes & ~bad;
+            }
           }
-        l[t] = l[t] * grow + sum;
-#pragma unroll
-        for (int i = 0; i < kDT; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[t][i][c] *= grow;
+        if (__ballot(any != 0)) {
+          spoilt = true;
+          if (lane < kKeys && pos != kNoKey) note_nans<D>(meta.nan_at, vbase + meta.off[which][lane], pos);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
       // O^T += V^T P^T, 32 keys at a time
 #pragma unroll
-      for (int i = 0; i < NK; i += 2) {
-        u32x4 p[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const f32x4 vs = *reinterpret_cast<const f32x4*>(&meta.vs[16 * (i + half) + 4 * quad]);
-            float f[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              f[c] = s[t][i + half][c] * vs[c];
-              if (edge && meta.pos[16 * (i + half) + 4 * quad + c] >= limit[t]) f[c] = 0.f;   // whatever the scale is
-            }
-            p[t][2 * half] = pack_f16(f[0], f[1]);
-            p[t][2 * half + 1] = pack_f16(f[2], f[3]);
-          }
-        uint32_t gone = 0;                                       // eight keys' bits: nobody sees them
-        if (edge)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) gone |= (meta.pos[16 * (i + c / 4) + 4 * quad + (c & 3)] == kNoKey ? 1u : 0u) << c;
+      for (int i = 0; i < NK; i += 2)
 #pragma unroll
         for (int dw = 0; dw < kDT / 4; ++dw) {
-          u32x2 x8[8];                                           // [key] -> places (0, 1) and (2, 3) of the dword
+          u32x4 f[4];
+          operands(i, dw, f);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t bytes = x.v[i + c / 4][c & 3][dw];
-            if (edge) bytes = (gone >> c) & 1u ? 0u : bytes;
-            x8[c] = widen4<1>(bytes);
-          }
+          for (int pl = 0; pl < 4; ++pl)
 #pragma unroll
-          for (int pl = 0; pl < 4; ++pl) {
-            u32x4 f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              f[c] = __builtin_amdgcn_perm(x8[2 * c + 1][pl / 2], x8[2 * c][pl / 2], pl & 1 ? 0x07060302u : 0x05040100u);
-            const int dt = 4 * dw + pl;
-            if (edge) {
-              // A NaN in V reaches the rows that see its key and no others: it is taken out of the
-              // product, and a second product counts, per output, the visible keys that hold one.
-              u32x4 bad;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) bad[c] = nan_halves(f[c]);
-              if (__ballot((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                  u32x4 vis, one;
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) {
-                    const int k0 = 16 * (i + c / 2) + 4 * quad + 2 * (c & 1);
-                    vis[c] = (meta.pos[k0] < limit[t] ? 0x3c00u : 0u) | (meta.pos[k0 + 1] < limit[t] ? 0x3c000000u : 0u);
-                    one[c] = bad[c] & 0x3c003c00u;
-                  }
-                  const f32x4 n = mfma16<1>(one, vis, f32x4{0, 0, 0, 0});
-#pragma unroll
-                  for (int c = 0; c < 4; ++c)
-                    if (n[c] > 0.f) o[t][dt][c] = __uint_as_float(0x7fc00000u);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) f[c] &= ~bad[c];
-              }
+            for (int t = 0; t < NT; ++t) {
+              o[t][4 * dw + pl] = mfma16<1>(f[pl], p[t][i / 2], o[t][4 * dw + pl]);
+              if constexpr (TYPE == 1) o[t][4 * dw + pl] = mfma16<1>(f[pl], p_low[t][i / 2], o[t][4 * dw + pl]);
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[t][dt] = mfma16<1>(f, p[t], o[t][dt]);
-          }
         }
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) copy_rows(which ^ 1, vbase, lds_v);
+      __builtin_amdgcn_sched_barrier(0);
+      return next;
     };
 
-    if (step0 < end) {
-      Data x0, x1;
-      int64_t pid = page_of(step0);
-      fetch(step0, pid, x0);
-      pid = step0 + 1 < end ? page_of(step0 + 1) : -1;
-      for (int step = step0; step < end; step += 2) {
-        if (step + 1 < end) {
-          fetch(step + 1, pid, x1);
-          pid = step + 2 < end ? page_of(step + 2) : -1;
-        }
-        compute(step, x0);
-        if (step + 1 >= end) break;
-        if (step + 2 < end) {
-          fetch(step + 2, pid, x0);
-          pid = step + 3 < end ? page_of(step + 3) : -1;
-        }
-        compute(step + 1, x1);
-      }
+    if (begin < end) {
+      wait_vmem<0>();
+      int pos = copy_scales(begin, 0);
+      copy_pages(begin + ways);
+      copy_rows(0, kbase, lds_k);
+      copy_rows(0, vbase, lds_v);
+      int which = 0;
+      for (int step = begin; step < end; step += ways, which ^= 1) pos = compute(step, which, pos, step + ways < end);
+      if (bad_page) raise_flag(a.status, ST_SLOT_PAGE);
     }
 
     // The lane holds, of row 16 t + col, places kDT * (4 quad + c) + dt.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (spoilt) {
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int from = meta.nan_at[kDT * (4 * quad + c) + dt];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (from < limit[t]) o[t][dt][c] = __uint_as_float(0x7fc00000u);
+        }
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       l[t] += __shfl_xor(l[t], 16);
       l[t] += __shfl_xor(l[t], 32);
-      const float inv = l[t] > 0.f ? 1.f / l[t] : (l[t] == 0.f ? 0.f : l[t]);     // a NaN sum stays one
-      if (!live[t]) continue;
+    }
+    const int64_t part0 = ((int64_t)(2 * slot + (first_of_share ? 0 : 1)) * H) * kM;       // the segment's place among the parts
+    // What is known of a row once all of its keys in the segment are: its lse, or its (m, l)
+    auto leave_sum = [&](int r, uint32_t token, int hd, float top, float sum) {
       if (whole) {
-        const uint64_t dst = (uint64_t)a.out + 2 * ((seq.first + tok[t]) * a.o_row + head[t] * a.o_head);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t y[kDT / 2];
-#pragma unroll
-          for (int dt = 0; dt < kDT; dt += 2)
-            y[dt / 2] = narrow<TYPE>(ldexpf(o[t][dt][c] * inv, r_exp - kPShift), ldexpf(o[t][dt + 1][c] * inv, r_exp - kPShift));
-          if constexpr (kDT == 8) gstore<u32x4>(dst + 2 * kDT * (4 * quad + c), u32x4{y[0], y[1], y[2], y[3]});
-          else gstore<u32x2>(dst + 2 * kDT * (4 * quad + c), u32x2{y[0], y[1]});
-        }
-        if (a.lse && quad == 0)
-          a.lse[(seq.first + tok[t]) * (int64_t)(H * G) + head[t]] = l[t] == 0.f ? kMinusInf : (m[t] + __log2f(l[t])) * 0.69314718055994530942f;
+        if (a.lse) a.lse[(seq.first + token) * (int64_t)(H * G) + hd] = sum == 0.f ? kMinusInf : (top + __log2f(sum)) * 0.69314718055994530942f;
       } else {
-        const int64_t part = ((int64_t)(2 * slot + (first_of_share ? 0 : 1)) * H + h) * kM + 16 * t + col;
-        const uint64_t dst = (uint64_t)(a.part_o + part * D);
+        const int64_t part = part0 + (int64_t)h * kM + r;
+        a.part_ml[2 * part] = top;
+        a.part_ml[2 * part + 1] = sum;
+      }
+    };
+    if (ways == 1) {
+      if (works)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (!live[t]) continue;
+          const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
+          if (quad == 0) leave_sum(16 * t + col, tok[t], head[t], m[t], l[t]);
+          const uint64_t dst = whole ? (uint64_t)a.out + 2 * ((seq.first + tok[t]) * a.o_row + head[t] * a.o_head)
+                                     : (uint64_t)(a.part_o + (part0 + (int64_t)h * kM + 16 * t + col) * D);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float y[kDT];
+#pragma unroll
+            for (int dt = 0; dt < kDT; ++dt) y[dt] = ldexpf(o[t][dt][c] * inv, r_exp - kPShift);
+            const int d = kDT * (4 * quad + c);
+            if (whole) {
+              if constexpr (kDT == 8)
+                gstore<u32x4>(dst + 2 * d, u32x4{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3]), narrow<TYPE>(y[4], y[5]), narrow<TYPE>(y[6], y[7])});
+              else
+                gstore<u32x2>(dst + 2 * d, u32x2{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3])});
+            } else {
+#pragma unroll
+              for (int dt = 0; dt < kDT; dt += 4) gstore<f32x4>(dst + 4 * (d + dt), f32x4{y[dt], y[dt + 1], y[dt + 2], y[dt + 3]});
+            }
+          }
+        }
+    } else {
+      // The waves of a head: each brings its sums to the common maximum and divides them by the common l; 16 rows at a time
+      // go through the waves' K and V space, which is free by now.
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (quad == 0) {
+          sums[wave][0][16 * t + col] = m[t];
+          sums[wave][1][16 * t + col] = l[t];
+        }
+      lds_barrier();
+      const int first = wave - way * (int)hw;                        // the head's first wave; the others follow hw apart
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int r = 16 * t + col;
+        float top = kMinusInf, sum = 0.f;
+        float mi[kWaves], li[kWaves];                                // all at once: a loop would wait for LDS at every turn
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+          const int from_wave = i < ways ? first + i * (int)hw : first;
+          mi[i] = sums[from_wave][0][r];
+          li[i] = i < ways ? sums[from_wave][1][r] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) top = fmaxf(top, mi[i]);
+        const float from = top == kMinusInf ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) sum += li[i] == 0.f ? 0.f : li[i] * exp2_fast(mi[i] - from);
+        const float mine = l[t] == 0.f ? 0.f : exp2_fast(m[t] - from) / sum;
+        float* space = reinterpret_cast<float*>(meta.kv);            // 16 rows of D floats
+        // a row's 16-byte pieces are XOR-ed with its number: sixteen lanes write sixteen rows at one place
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int dt = 0; dt < kDT; dt += 4) {
             f32x4 y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = ldexpf(o[t][dt + k][c] * inv, r_exp - kPShift);
-            gstore<f32x4>(dst + 4 * (kDT * (4 * quad + c) + dt), y);
+            for (int k = 0; k < 4; ++k) y[k] = ldexpf(o[t][dt + k][c] * mine, r_exp - kPShift);
+            *reinterpret_cast<f32x4*>(space + col * D + 4 * (((kDT * (4 * quad + c) + dt) / 4) ^ (col & (D / 4 - 1)))) = y;
           }
-        if (quad == 0) {
-          a.part_ml[2 * part] = m[t];
-          a.part_ml[2 * part + 1] = l[t];
+        if (works && way == 0 && quad == 0 && live[t]) leave_sum(r, tok[t], head[t], top, sum);
+        lds_barrier();
+        // way i of the head adds up rows i, i + ways, ...; four places a lane
+        constexpr int kRowLanes = D / 4, kRowsAtOnce = 64 / kRowLanes;
+        const int j = lane % kRowLanes;
+        for (int rr = way * kRowsAtOnce + lane / kRowLanes; works && rr < 16 && 16 * t + rr < rows; rr += ways * kRowsAtOnce) {
+          f32x4 y = {0, 0, 0, 0};
+          f32x4 x[kWaves];
+#pragma unroll
+          for (int i = 0; i < kWaves; ++i)
+            x[i] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(metas[i < ways ? first + i * (int)hw : first].kv) + rr * D + 4 * (j ^ (rr & (D / 4 - 1))));
+#pragma unroll
+          for (int i = 0; i < kWaves; ++i)
+            if (i < ways) y += x[i];
+          const uint32_t row = (uint32_t)(tile * kM + 16 * t + rr), tk = divide(row, a.group);
+          if (whole)
+            gstore<u32x2>((uint64_t)a.out + 2 * ((seq.first + tk) * a.o_row + (h * G + (int)(row - tk * G)) * a.o_head + 4 * j),
+                          u32x2{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3])});
+          else
+            gstore<f32x4>((uint64_t)(a.part_o + (part0 + (int64_t)h * kM + 16 * t + rr) * D + 4 * j), y);
         }
+        lds_barrier();                                             // before the space is written again
       }
     }
     at += count;
     local += count;
   }
+  if (a.slots > 1 && h0 == 0 && tid == 0) a.part_join[slot] = join;
 }
 
 // Joins `n` partial results of one row: weights l_i 2^(m_i - max m). A wave does a row; `at(i)` is the index of the
@@ -538,14 +710,22 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int lane, int n, F
     }
     sum += w;
     const int here = n - base < 64 ? n - base : 64;
-#pragma unroll 4
-    for (int i = 0; i < here; i += kParts) {
-      const float wi = __shfl(w, i + sub);
-      if (i + sub < here && wi != 0.f) {
-        const f32x4 y = gload<f32x4>((uint64_t)(a.part_o + at(base + i + sub) * D + d));
+    constexpr int kAtOnce = 8;              // loads under way
+    for (int i0 = 0; i0 < here; i0 += kParts * kAtOnce) {
+      f32x4 y[kAtOnce];
+      float wi[kAtOnce];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] += wi * y[c];
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = i0 + u * kParts + sub, in = i < here ? i : here - 1;
+        wi[u] = __shfl(w, in);
+        wi[u] = i < here ? wi[u] : 0.f;
+        y[u] = gload<f32x4>((uint64_t)(a.part_o + at(base + in) * D + d));
       }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (wi[u] != 0.f)                   // what a part without weight holds was never written
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] += wi[u] * y[u][c];
     }
   }
   for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
@@ -560,34 +740,19 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int lane, int n, F
   if (a.lse && lane == 0) a.lse[row * q_heads + head] = sum == 0.f ? kMinusInf : (top + __log2f(sum)) * 0.69314718055994530942f;
 }
 
-// One workgroup per (slot, KV head): joins the tile that begins in the slot's share and ends behind it, if
-// there is one. The parts are summed in the order of the shares, so the result does not depend on timing.
-template <int D, int TYPE, int NT, int NK>
+// A wave per row, a workgroup per (slot, KV head) and four rows: joins the tile that begins in the slot's share and ends behind it, if
+// there is one (the slot has left word). The parts are summed in the order of the shares, so the result does not depend on timing.
+template <int D, int TYPE, int M>
 __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
-  using C = Few<D, TYPE, NT, NK>;
-  constexpr int kM = C::kM, kKeys = C::kKeys;
   const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int H = a.layer.heads, G = (int)a.group.d;
-  const int h = blockIdx.x % H, slot = blockIdx.x / H;
-  const int64_t total = line_length<kM, kKeys>(a, lane);
-  const Line line = share_of(total, a.slots, a.min_steps, slot);
-  if (line.begin >= line.end || line.end >= total) return;
-  int64_t local = 0;
-  const int64_t b = seq_at<kM, kKeys>(a, line.end - 1, lane, &local);
-  if (b >= a.seq.n_seqs) return;
-  const Seq seq = read_seq(a.seq, b);
-  const int steps = steps_of(seq, kKeys);
-  const int tile = (int)(local / steps);
-  const int64_t tile_begin = line.end - 1 - (local - (int64_t)tile * steps), tile_end = tile_begin + steps;
-  if (tile_end <= line.end || tile_begin < line.begin) return;
-  const int last = slot_of(total, a.slots, a.min_steps, tile_end - 1);
-  const int first_index = 2 * slot + (tile_begin == line.begin ? 0 : 1);
-  const int64_t left = (int64_t)seq.n * G - (int64_t)tile * kM;
-  const int rows = (int)(left < kM ? left : kM);
-  for (int r = wave; r < rows; r += 4) {
-    const uint32_t row = (uint32_t)(tile * kM + r), tok = divide(row, a.group);
-    auto at = [&](int i) { return ((int64_t)(i == 0 ? first_index : 2 * (slot + i)) * H + h) * kM + r; };
-    join_row<D, TYPE>(a, lane, last - slot + 1, at, seq.first + tok, h * G + (int)(row - tok * G), H * G);
+  const int slot = blockIdx.x / H, h = blockIdx.x - slot * H;
+  const JoinHead j = a.part_join[slot];
+  const int r = blockIdx.y * 4 + wave;
+  if (r < j.rows) {
+    const uint32_t row = (uint32_t)(j.tile * M + r), tok = divide(row, a.group);
+    auto at = [&](int i) { return ((int64_t)(i == 0 ? j.first_index : 2 * (slot + i)) * H + h) * M + r; };
+    join_row<D, TYPE>(a, lane, j.parts, at, j.first_row + tok, h * G + (int)(row - tok * G), H * G);
   }
 }
 
@@ -616,15 +781,6 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ int64_t first_tile(const AttendArgs& a, int64_t b) {
-  int64_t q = b;
-  if (a.seq.q_starts) {
-    q = a.seq.q_starts[b];
-    q = q < 0 ? 0 : q > a.seq.n_rows ? a.seq.n_rows : q;
-  }
-  return q * a.group.d / kManyRows + b;
-}
-
 template <int D, int TYPE>
 __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArgs a) {
   constexpr int kKeys = kManyKeys;
@@ -637,6 +793,8 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     int pos[kKeys];
     int gone;
   };
+  __shared__ int nan_at[D];                       // by place: the first key with a NaN in V that not every row sees
+  __shared__ int spoilt;
   __shared__ u32x4 k_lds[2][kKeys * kChunks];
   __shared__ u32x4 v_lds[2][D * 8];
   __shared__ Meta metas[3];
@@ -651,10 +809,10 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   const int G = (int)a.group.d;
   const int P = (int)a.layer.page_tokens.d;
 
-  const int64_t b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile(a, i); });
+  const int64_t b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile<kManyRows>(a, i); });
   if (h == 0 && part == 0 && slot < a.seq.n_seqs && tid == 0 && !read_seq(a.seq, slot).ok) raise_flag(a.status, ST_SLOT_SRC);
   const Seq seq = read_seq(a.seq, b);
-  const int64_t tile64 = slot - first_tile(a, b);
+  const int64_t tile64 = slot - first_tile<kManyRows>(a, b);
   const int64_t n_rows = (int64_t)seq.n * G;
   if (!seq.ok || tile64 < 0 || tile64 * kManyRows >= n_rows) return;
   const int tile = uni((int)tile64);
@@ -681,6 +839,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   const int wave_last = 32 * wave + 31 < rows ? 32 * wave + 31 : rows - 1;
   const int wave_seen = uni(32 * wave < rows ? sees(row0 + wave_last) : 0);
   const int wave_all = uni(32 * wave < rows ? sees(row0 + 32 * wave) : 0);
+  const int all = uni(sees(row0));                 // keys that every row of the tile sees
   u32x4 q[D / 16];
   {
     const uint64_t src = (uint64_t)a.q + 2 * ((seq.first + tok) * a.q_row + head * a.q_head);
@@ -749,7 +908,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       }
     }
   };
-  auto put = [&](int buf, const Meta& m) {
+  auto put = [&](int t, int buf, const Meta& m) {
     if (!brings_v) {
       constexpr int kRowLanes = D / 16;
 #pragma unroll
@@ -763,10 +922,25 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       }
     } else {
       const int g = p >> 4, c16 = p & 15;
-      uint32_t gone = 0;
-      if (m.gone)
+      if ((t + 1) * kKeys > all || m.gone) {
+        // bytes of keys that nobody sees become zero, and so does a NaN: the rows that see its key get it at the end
+        uint32_t any = 0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) gone |= (m.pos[16 * (g >> 1) + 8 * (c >> 2) + 4 * (g & 1) + (c & 3)] == kNoKey ? 1u : 0u) << c;
+        for (int c = 0; c < 8; ++c) {
+          const int pos = m.pos[16 * (g >> 1) + 8 * (c >> 2) + 4 * (g & 1) + (c & 3)];
+#pragma unroll
+          for (int dw = 0; dw < kVB / 4; ++dw) {
+            const int r0 = kVB == 8 ? c / 2 : c / 4, r1 = kVB == 8 ? 2 * (c & 1) + dw : c & 3;
+            const uint32_t bytes = pos == kNoKey ? 0 : raw[r0][r1], bad = nan_bytes(bytes);
+            any |= bad;
+            raw[r0][r1] = bytes & ~bad;
+          }
+        }
+        if (__ballot(any != 0)) {
+          spoilt = 1;
+          if (m.pos[lane] != kNoKey) note_nans<D>(nan_at, vbase + m.off[lane], m.pos[lane]);
+        }
+      }
 #pragma unroll
       for (int dw = 0; dw < kVB / 4; ++dw) {
         u32x2 x8[8];
@@ -775,7 +949,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
           uint32_t bytes;
           if constexpr (kVB == 8) bytes = raw[c / 2][2 * (c & 1) + dw];
           else bytes = raw[c / 4][c & 3];
-          x8[c] = widen4<1>((gone >> c) & 1u ? 0u : bytes);
+          x8[c] = widen4<1>(bytes);
         }
 #pragma unroll
         for (int pl = 0; pl < 4; ++pl) {
@@ -878,29 +1052,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
           const int d = 32 * dt + col;
-          u32x4 f = v_lds[buf][d * 8 + (g ^ ((d >> 1) & 7))];
-          if (edge) {
-            u32x4 bad;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) bad[c] = nan_halves(f[c]);
-            if (__ballot((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
-              u32x4 vis, one;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const int k0 = 32 * kb + 16 * s2 + 8 * (c >> 1) + 4 * half + 2 * (c & 1);
-                vis[c] = (meta.pos[k0] < limit ? 0x3c00u : 0u) | (meta.pos[k0 + 1] < limit ? 0x3c000000u : 0u);
-                one[c] = bad[c] & 0x3c003c00u;
-                f[c] &= ~bad[c];
-              }
-              f32x16 n;
-#pragma unroll
-              for (int c = 0; c < 16; ++c) n[c] = 0.f;
-              n = mfma32<1>(one, vis, n);
-#pragma unroll
-              for (int c = 0; c < 16; ++c)
-                if (n[c] > 0.f) o[dt][c] = __uint_as_float(0x7fc00000u);
-            }
-          }
+          const u32x4 f = v_lds[buf][d * 8 + (g ^ ((d >> 1) & 7))];
           o[dt] = mfma32<1>(f, pf, o[dt]);
         }
       }
@@ -915,9 +1067,11 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       if (t0 + 1 < t1) put_meta(metas[1], look_up(t0 + 1, page_of(t0 + 1)));
       if (t0 + 2 < t1) pid = page_of(t0 + 2);
     }
+    for (int d = tid; d < D; d += 256) nan_at[d] = kNoKey;
+    if (tid == 0) spoilt = 0;
     __syncthreads();
     bring(metas[0]);
-    put(0, metas[0]);
+    put(t0, 0, metas[0]);
     __syncthreads();
     int mi = 0;
     for (int t = t0; t < t1; ++t) {
@@ -929,11 +1083,17 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         if (t + 3 < t1) pid = page_of(t + 3);
       }
       if (t * kKeys < wave_seen) compute(t, buf, metas[mi]);
-      if (t + 1 < t1) put(buf ^ 1, metas[m1]);
+      if (t + 1 < t1) put(t + 1, buf ^ 1, metas[m1]);
       if (wave == 0 && t + 2 < t1) put_meta(metas[m2], next);
       __syncthreads();
       mi = m1;
     }
+    if (spoilt)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (nan_at[32 * i + 8 * (e / 4) + 4 * half + (e & 3)] < limit) o[i][e] = __uint_as_float(0x7fc00000u);
   }
 
   l_run += __shfl_xor(l_run, 32);
@@ -983,9 +1143,9 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
   const uint32_t rest = id / (kManyRows / 4);
   const int h = (int)(rest % (uint32_t)H);
   const int64_t slot = rest / (uint32_t)H;
-  const int64_t b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile(a, i); });
+  const int64_t b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile<kManyRows>(a, i); });
   const Seq seq = read_seq(a.seq, b);
-  const int64_t tile = slot - first_tile(a, b);
+  const int64_t tile = slot - first_tile<kManyRows>(a, b);
   if (!seq.ok || tile < 0 || tile * kManyRows + r >= (int64_t)seq.n * G) return;
   const uint32_t row = (uint32_t)(tile * kManyRows + r), tok = divide(row, a.group);
   auto at = [&](int i) { return ((slot * H + h) * a.slots + i) * kManyRows + r; };
@@ -997,15 +1157,25 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
   AttendPlan p = {};
   const int64_t all = n_rows * group;                      // rows of one KV head
   const int64_t mean = (all + n_seqs - 1) / n_seqs;
-  if (mean <= 64) {
+  const int m = mean <= 16 ? 16 : mean <= 32 ? 32 : 64, keys = m == 16 ? 64 : 32;
+  if (mean <= 64 && (all / m + n_seqs) * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
     p.form = mean <= 16 ? ATTEND_FEW_16 : mean <= 32 ? ATTEND_FEW_32 : ATTEND_FEW_64;
-    p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-    // as many waves as the chip holds at once: 256 CUs x 4 SIMDs x 2 (one where a wave has all registers)
-    const int64_t waves = p.form == ATTEND_FEW_16 ? 2048 : 1024;
-    int64_t slots = waves / heads;
-    p.slots = (int32_t)(slots < 1 ? 1 : slots);
-    p.min_steps = 1;
-    p.part_rows = 2 * (int64_t)p.slots * heads * p.rows;
+    p.rows = m;
+    p.tiles = all / m + n_seqs;
+    p.tiles = all / m + n_seqs;
+    const int waves = m == 64 ? 4 : 8;
+    p.heads_per_group = heads < waves ? heads : waves;
+    if (max_len <= 2048) {
+      // a workgroup per tile; with few of them a head gets more waves
+      while (p.heads_per_group > 1 && p.tiles * ((heads + p.heads_per_group - 1) / p.heads_per_group) < 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
+      p.slots = 0;
+    } else {
+      // one workgroup for each of the 256 CUs, which is what one holds of this size
+      const int64_t slots = 256 / ((heads + p.heads_per_group - 1) / p.heads_per_group);
+      p.slots = (int32_t)(slots < 1 ? 1 : slots);
+    }
+    p.min_steps = waves / p.heads_per_group;
+    p.part_rows = p.slots > 1 ? 2 * (int64_t)p.slots * heads * p.rows : 0;
   } else {
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
@@ -1021,9 +1191,9 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
 
 template <int D, int TYPE, int NT, int NK>
 static hipError_t launch_few(const AttendPlan& p, const AttendArgs& a, hipStream_t s) {
-  const int64_t waves = (int64_t)p.slots * a.layer.heads;
-  hipLaunchKernelGGL((fp8_attend_few_kernel<D, TYPE, NT, NK>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, a);
-  if (p.slots > 1) hipLaunchKernelGGL((fp8_join_few_kernel<D, TYPE, NT, NK>), dim3((uint32_t)waves), dim3(256), 0, s, a);
+  const int64_t groups = (p.slots > 0 ? p.slots : p.tiles) * ((a.layer.heads + p.heads_per_group - 1) / p.heads_per_group);
+  hipLaunchKernelGGL((fp8_attend_few_kernel<D, TYPE, NT, NK>), dim3((uint32_t)groups), dim3(64 * Few<D, TYPE, NT, NK>::kWaves), 0, s, a);
+  if (p.slots > 1) hipLaunchKernelGGL((fp8_join_few_kernel<D, TYPE, 16 * NT>), dim3((uint32_t)(p.slots * a.layer.heads), 4 * NT), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -1046,6 +1216,7 @@ hipError_t launch_fp8_attend(const AttendPlan& p, int head_dim, int type, const 
   a.slots = p.slots;
   a.min_steps = p.min_steps;
   a.tiles = p.tiles;
+  a.heads_per_group = p.heads_per_group;
   if (head_dim == 128) return type == 0 ? launch_form<128, 0>(p, a, stream) : launch_form<128, 1>(p, a, stream);
   return type == 0 ? launch_form<64, 0>(p, a, stream) : launch_form<64, 1>(p, a, stream);
 }

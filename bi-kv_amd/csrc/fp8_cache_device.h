@@ -31,41 +31,14 @@ __device__ __forceinline__ void gstore_nt(uint64_t addr, T v) {
 }
 
 __device__ __forceinline__ void raise_flag(uint32_t* status, int slot) {
-  *reinterpret_cast<volatile uint32_t*>(status + slot) = 1u;
+  *(volatile BIKV_G uint32_t*)(status + slot) = 1u;
 }
-
-__device__ __forceinline__ uint32_t divide(uint32_t n, const FastDiv& f) { return (uint32_t)((n * f.mul) >> f.shift); }
 
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uni64(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ int64_t shfl64(int64_t x, int src) {
-  const uint32_t lo = __shfl((uint32_t)x, src);
-  const uint32_t hi = __shfl((uint32_t)((uint64_t)x >> 32), src);
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ int64_t shfl_up64(int64_t x, int by) {
-  const uint32_t lo = __shfl_up((uint32_t)x, by);
-  const uint32_t hi = __shfl_up((uint32_t)((uint64_t)x >> 32), by);
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-  for (int m = 32; m > 0; m >>= 1) {
-    const uint32_t lo = __shfl_xor((uint32_t)x, m);
-    const uint32_t hi = __shfl_xor((uint32_t)((uint64_t)x >> 32), m);
-    x += (int64_t)(((uint64_t)hi << 32) | lo);
-  }
-  return x;
-}
-__device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {   // inclusive
-  for (int m = 1; m < 64; m <<= 1) {
-    const int64_t y = shfl_up64(x, m);
-    if (lane >= m) x += y;
-  }
-  return x;
 }
 
 // A sequence as the kernels use it. One whose numbers make no sense (a negative length, more tokens than

@@ -5,21 +5,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-namespace bikv {
+#include "host_logic/fp8_logic.h"
 
-// n / d for 0 <= n < 2^31 without a division: (n * mul) >> shift with mul = floor(2^shift / d) + 1,
-// shift = 31 + ceil(log2 d). The multiplier is too large by e <= 1 (in units of 2^shift / d), and
-// n * e * d < 2^31 * 2^ceil(log2 d), so the quotient is exact.
-struct FastDiv {
-  uint32_t d;
-  uint32_t shift;
-  uint64_t mul;
-};
-inline FastDiv fast_div(uint32_t d) {
-  uint32_t s = 0;
-  while ((uint64_t(1) << s) < d) ++s;
-  return {d, 31 + s, (uint64_t(1) << (31 + s)) / d + 1};
-}
+namespace bikv {
 
 // The sequences of one call: where their pages are, how long they are, which rows of the caller's
 // tensors are theirs. All arrays are device memory.
@@ -59,6 +47,15 @@ struct AppendArgs {
 // type: 0 = bf16, 1 = fp16
 hipError_t launch_fp8_append(int head_dim, int type, const AppendArgs& a, hipStream_t stream);
 
+// Few rows: what a slot says of the row tile that begins in its share and ends in a later one.
+struct JoinHead {
+  int64_t first_row;         // of the tile's sequence
+  int32_t tile;
+  int32_t rows;              // 0: there is none
+  int32_t parts;
+  int32_t first_index;       // of its first part; the i-th other one is 2 * (slot + i)
+};
+
 struct AttendArgs {
   SeqArgs seq;
   LayerArgs layer;
@@ -71,9 +68,11 @@ struct AttendArgs {
   float scale_log2;          // softmax scale * log2(e)
   float* part_o;             // partial results, see the kernels
   float* part_ml;
-  int32_t slots;             // few rows: shares the work is cut into; many rows: parts a tile's keys are cut into
+  JoinHead* part_join;       // few rows: one per slot
+  int32_t slots;             // few rows: shares the work is cut into, 0 = a workgroup per tile; many rows: parts a tile's keys are cut into
   int32_t min_steps;         // few rows: key steps a share has at least
-  int64_t tiles;             // many rows: row tiles of the launch
+  int32_t heads_per_group;   // few rows: KV heads of a workgroup
+  int64_t tiles;             // row tiles of the launch
   uint32_t* status;
 };
 enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_FEW_64 = 2, ATTEND_MANY = 3 };
@@ -82,6 +81,7 @@ struct AttendPlan {
   int rows;                  // rows of a tile
   int32_t slots;
   int32_t min_steps;
+  int32_t heads_per_group;
   int64_t tiles;
   int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
 };
