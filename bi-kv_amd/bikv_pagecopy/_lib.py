@@ -88,20 +88,6 @@ class FP8CacheDesc(C.Structure):
     ]
 
 
-class SeqBatchDesc(C.Structure):
-    _fields_ = [
-        ("page_table", C.c_void_p),
-        ("page_table_stride", C.c_int64),
-        ("max_pages", C.c_int64),
-        ("kv_lens", C.c_void_p),
-        ("q_starts", C.c_void_p),
-        ("n_seqs", C.c_int64),
-        ("n_rows", C.c_int64),
-        ("dtype", C.c_int32),
-        ("reserved", C.c_int32),
-    ]
-
-
 class AllocInfo(C.Structure):
     _fields_ = [("bytes", C.c_int64), ("chunk_bytes", C.c_int64), ("n_chunks", C.c_int32),
                 ("n_other_half", C.c_int32), ("n_fillers", C.c_int32), ("n_reprobed", C.c_int32),
@@ -172,10 +158,10 @@ _SIGNATURES = {
     "bikv_copy_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "bikv_fp8_cache_create": (C.c_int, [C.POINTER(FP8CacheDesc), C.POINTER(C.c_void_p)]),
     "bikv_fp8_cache_destroy": (C.c_int, [C.c_void_p]),
-    "bikv_fp8_append": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SeqBatchDesc), C.c_void_p, C.c_int64, C.c_int64,
+    "bikv_fp8_append": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                   C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
-    "bikv_fp8_attend_workspace": (C.c_int64, [C.c_void_p, C.POINTER(SeqBatchDesc), C.c_int32]),
-    "bikv_fp8_attend": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SeqBatchDesc), C.c_void_p, C.c_int64, C.c_int64,
+    "bikv_fp8_attend_workspace": (C.c_int64, [C.c_void_p, C.c_void_p, C.c_int32]),
+    "bikv_fp8_attend": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                   C.c_int32, C.c_int32, C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
                                   C.c_void_p, C.c_int64, C.c_void_p]),
     "bikv_stager_create": (C.c_int, [C.c_int, C.c_int64, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),

@@ -19,13 +19,15 @@ with the sequences described by device tensors, so that a captured graph replays
 """
 import ctypes as C
 import math
+import struct
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from .pool import PagedKVPool, _stream_ptr
+from .pool import PagedKVPool, current_raw_stream
 
+_SEQ_BATCH = struct.Struct("=7q2i")          # bikv_seq_batch
 _TYPES = {torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_FP16}
 
 
@@ -84,45 +86,58 @@ class FP8KVCache:
         h = C.c_void_p()
         _lib.check(_lib.load().bikv_fp8_cache_create(C.byref(d), C.byref(h)))
         self._h = h
+        self._lib = _lib.load()
+        self._default_scale = 1.0 / math.sqrt(self.head_dim)
+        self._workspace = {}
         self.pool = PagedKVPool.from_planes(planes, scales)      # keeps the tensors alive, too
 
     # ---- arguments ----------------------------------------------------------------------------
-    def _rows(self, name, t, heads=None):
-        if t.device != self.device:
-            raise RuntimeError(f"{name} must be on the cache's device")
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise RuntimeError(f"{name} must be [rows, {heads if heads is not None else 'heads'}, {self.head_dim}], got {list(t.shape)}")
-        if t.dtype not in _TYPES:
-            raise RuntimeError(f"{name} must be bfloat16 or float16")
-        if t.stride(2) != 1 and t.numel():
+    # A step calls these once per layer, so the checks are few expressions and what is wrong is found out afterwards.
+    def _rows(self, name, t, heads):
+        """Strides (row, head) of a [rows, heads, head_dim] tensor the kernels can read; raises for any other."""
+        shape, stride = t.shape, t.stride()
+        if (t.device != self.device or len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads)
+                or t.dtype not in _TYPES or stride[2] != 1 and t.numel()):
+            if t.device != self.device:
+                raise RuntimeError(f"{name} must be on the cache's device")
+            if t.dtype not in _TYPES:
+                raise RuntimeError(f"{name} must be bfloat16 or float16")
+            if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+                raise RuntimeError(f"{name} must be [rows, {heads if heads is not None else 'heads'}, {self.head_dim}], got {list(shape)}")
             raise RuntimeError(f"{name}: the values of a head must be contiguous")
-        return t
+        return stride
 
     def _batch(self, rows, page_table, kv_lens, q_starts):
-        for name, t, dim in (("page_table", page_table, 2), ("kv_lens", kv_lens, 1), ("q_starts", q_starts, 1)):
-            if t is None and name == "q_starts":
-                continue
-            if t.device != self.device or t.dtype != torch.int64 or t.dim() != dim:
-                raise RuntimeError(f"{name} must be a {dim}-D int64 tensor on the cache's device")
-            if t.numel() and t.stride(-1) != 1 and t.shape[-1] > 1:
-                raise RuntimeError(f"{name} must be contiguous along its last dimension")
-        n = kv_lens.shape[0]
-        if page_table.shape[0] != n:
-            raise RuntimeError("page_table and kv_lens differ in their number of sequences")
-        if q_starts is not None and q_starts.shape[0] != n + 1:
-            raise RuntimeError("q_starts must have one entry more than there are sequences")
-        if q_starts is None and rows.shape[0] != n:
-            raise RuntimeError(f"without q_starts every sequence has one row: {rows.shape[0]} rows, {n} sequences")
-        if page_table.shape[0] > 1 and page_table.shape[1] and page_table.stride(0) < page_table.shape[1]:
+        """The bikv_seq_batch of a call, as bytes; raises for arrays that are not what it says."""
+        n_rows, dtype = rows.shape[0], rows.dtype
+        shape, stride, lens_shape = page_table.shape, page_table.stride(), kv_lens.shape
+        dev, i64 = self.device, torch.int64
+        if (page_table.dtype != i64 or page_table.device != dev or len(shape) != 2 or stride[1] != 1 and shape[1] > 1
+                or stride[0] < shape[1] and shape[0] > 1):
+            self._refuse_array("page_table", page_table, 2)
             raise RuntimeError("page_table's rows must not overlap")
-        d = _lib.SeqBatchDesc()
-        d.page_table = page_table.data_ptr()
-        d.max_pages = page_table.shape[1]
-        d.page_table_stride = max(page_table.stride(0), page_table.shape[1])
-        d.kv_lens = kv_lens.data_ptr()
-        d.q_starts = q_starts.data_ptr() if q_starts is not None else None
-        d.n_seqs, d.n_rows, d.dtype = n, rows.shape[0], _TYPES[rows.dtype]
-        return d
+        if kv_lens.dtype != i64 or kv_lens.device != dev or len(lens_shape) != 1 or kv_lens.stride(0) != 1 and lens_shape[0] > 1:
+            self._refuse_array("kv_lens", kv_lens, 1)
+        n = lens_shape[0]
+        if shape[0] != n:
+            raise RuntimeError("page_table and kv_lens differ in their number of sequences")
+        starts = 0
+        if q_starts is not None:
+            if q_starts.dtype != i64 or q_starts.device != dev or q_starts.dim() != 1 or q_starts.stride(0) != 1 and q_starts.shape[0] > 1:
+                self._refuse_array("q_starts", q_starts, 1)
+            if q_starts.shape[0] != n + 1:
+                raise RuntimeError("q_starts must have one entry more than there are sequences")
+            starts = q_starts.data_ptr()
+        elif n_rows != n:
+            raise RuntimeError(f"without q_starts every sequence has one row: {n_rows} rows, {n} sequences")
+        return _SEQ_BATCH.pack(page_table.data_ptr(), stride[0] if stride[0] > shape[1] else shape[1], shape[1], kv_lens.data_ptr(), starts, n, n_rows,
+                               _TYPES[dtype], 0)
+
+    def _refuse_array(self, name, t, dim):
+        if t.device != self.device or t.dtype != torch.int64 or t.dim() != dim:
+            raise RuntimeError(f"{name} must be a {dim}-D int64 tensor on the cache's device")
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise RuntimeError(f"{name} must be contiguous along its last dimension")
 
     # ---- the two calls ------------------------------------------------------------------------
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -132,15 +147,14 @@ class FP8KVCache:
         its new values; a page with older tokens keeps its scale as long as the new values fit, and is rounded to
         a larger one when they do not. A page may be written by one sequence of a call only (fork a shared last
         page with PagedKVPool.copy_pages first)."""
-        self._rows("k", k, self.kv_heads)
-        self._rows("v", v, self.kv_heads)
+        ks, vs = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise RuntimeError("k and v must share shape and dtype")
-        d = self._batch(k, page_table, kv_lens, q_starts)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().bikv_fp8_append(
-                self._h, layer, C.byref(d), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                _stream_ptr(self.device)))
+        batch = self._batch(k, page_table, kv_lens, q_starts)
+        rc = self._lib.bikv_fp8_append(self._h, layer, batch, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                       current_raw_stream(self._device_index))
+        if rc < 0:
+            _lib.check(rc)
 
     def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                q_starts: Optional[torch.Tensor] = None, causal: bool = True, softmax_scale: Optional[float] = None,
@@ -150,32 +164,40 @@ class FP8KVCache:
         sequence's n rows sees the tokens up to its own (kv_len - n + t + 1 of them), without it all kv_len. Rows that see
         nothing get zeros (lse -inf). Returns out, or (out, lse) with lse [rows, q_heads] float32, the natural
         logarithm of the softmax's sum (what results over different pages are merged by). Rows behind the last
-        sequence's are not written: in an `out` (and lse) made here they hold whatever the memory held."""
-        self._rows("q", q)
-        d = self._batch(q, page_table, kv_lens, q_starts)
+        sequence's are not written: in an `out` (and lse) made here they hold whatever the memory held. `out` must lie in
+        other memory than q."""
+        qs, shape = self._rows("q", q, None), q.shape
+        batch = self._batch(q, page_table, kv_lens, q_starts)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(shape)
+            os = out.stride()
         else:
-            self._rows("out", out)
-            if out.shape != q.shape or out.dtype != q.dtype:
+            os = self._rows("out", out, None)
+            if out.shape != shape or out.dtype != q.dtype:
                 raise RuntimeError("out must have q's shape and dtype")
-            (s0, s1), (n0, n1) = out.stride()[:2], out.shape[:2]
+            (s0, s1, _), (n0, n1, _) = os, shape
             if out.numel() and not ((n1 == 1 or s1 >= self.head_dim) and (n0 == 1 or s0 >= s1 * (n1 - 1) + self.head_dim) or
                                     (n0 == 1 or s0 >= self.head_dim) and (n1 == 1 or s1 >= s0 * (n0 - 1) + self.head_dim)):
                 raise RuntimeError("out's rows overlap")
             if out.numel() and out.data_ptr() < _end(q) and q.data_ptr() < _end(out):
                 raise RuntimeError("out must not share memory with q")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        lib = _lib.load()
-        need = _lib.check(lib.bikv_fp8_attend_workspace(self._h, C.byref(d), q.shape[1]))
-        # from torch's allocator on the current stream: a call of its own in flight elsewhere, or in another graph, has another one
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
-        with torch.cuda.device(self.device):
-            _lib.check(lib.bikv_fp8_attend(
-                self._h, layer, C.byref(d), q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], int(bool(causal)), scale,
-                out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if lse is not None else None,
-                ws.data_ptr() if ws is not None else None, need, _stream_ptr(self.device)))
+        heads = shape[1]
+        lse = q.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
+        key = (shape[0], heads, page_table.shape)
+        need = self._workspace.get(key)
+        if need is None:                     # a size that follows from these numbers alone
+            need = _lib.check(self._lib.bikv_fp8_attend_workspace(self._h, batch, heads))
+            if len(self._workspace) >= 1024:
+                self._workspace.clear()
+            self._workspace[key] = need
+        # from torch's allocator on the current stream: a call in flight elsewhere, or in another graph, has another one
+        ws = q.new_empty(need // 2) if need else None
+        rc = self._lib.bikv_fp8_attend(
+            self._h, layer, batch, q.data_ptr(), qs[0], qs[1], heads, 1 if causal else 0,
+            self._default_scale if softmax_scale is None else softmax_scale, out.data_ptr(), os[0], os[1],
+            lse.data_ptr() if return_lse else None, ws.data_ptr() if need else None, need, current_raw_stream(self._device_index))
+        if rc < 0:
+            _lib.check(rc)
         return (out, lse) if return_lse else out
 
     def check(self):

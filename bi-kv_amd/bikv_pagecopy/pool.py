@@ -28,6 +28,11 @@ def _stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def current_raw_stream(device_index: int) -> int:
+    """The current stream's handle as a number; a stream object for every call would cost more than a small launch."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 class PageBatch:
     """Index arrays of one batch of requests, resident on the device.
 
@@ -128,6 +133,8 @@ class PagedKVPool:
             d.scale_tile_bytes = int(scale_tile_bytes)
             d.scale_page_stride_bytes = int(scale_page_stride_bytes)
         self._device_index = d.device
+        self._tensor_device = torch.device("cuda", d.device)
+        self._lib = lib
         h = C.c_void_p()
         _lib.check(lib.bikv_pool_create(C.byref(d), C.byref(h)))
         self._h = h
@@ -288,14 +295,15 @@ class PagedKVPool:
         stream (asynchronous): a fork's partly filled last page, a compaction's moves. Both are int64 device
         tensors, as page_moves makes them from host lists; ids made on the device must satisfy what
         it checks (an id outside the pool is skipped and reported by check(), the others are the caller's word)."""
-        for name, t in (("src_ids", src_ids), ("dst_ids", dst_ids)):
-            if t.device != self.device or t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
-                raise RuntimeError(f"{name} must be a contiguous 1-D int64 tensor on the pool's device")
-        if src_ids.numel() != dst_ids.numel():
+        for t in (src_ids, dst_ids):
+            if t.device != self._tensor_device or t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise RuntimeError("src_ids and dst_ids must be contiguous 1-D int64 tensors on the pool's device")
+        n = src_ids.shape[0]
+        if dst_ids.shape[0] != n:
             raise RuntimeError("src_ids and dst_ids differ in length")
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().bikv_copy_pages(self._h, src_ids.data_ptr(), dst_ids.data_ptr(), src_ids.numel(),
-                                                   _stream_ptr(self.device)))
+        rc = self._lib.bikv_copy_pages(self._h, src_ids.data_ptr(), dst_ids.data_ptr(), n, current_raw_stream(self._device_index))
+        if rc < 0:
+            _lib.check(rc)
 
     def check(self):
         """Synchronises the current stream and raises if a kernel rejected a page id or slot."""

@@ -1,7 +1,7 @@
 """The 8-bit cache on the GPU: append byte for byte, attention against a plain computation in 64 bits."""
 import math
+import struct
 
-import numpy as np
 import pytest
 import torch
 
@@ -623,7 +623,6 @@ def test_the_pool_beside_the_cache_moves_its_pages(bk, cuda):
 
 
 def test_refusals(bk, lib, cuda):
-    import ctypes as C
     from bikv_pagecopy import _lib
     w = World(bk, cuda, [40, 20], [1, 1], H=2, Hq=4, seed=36, ragged=False)
     k, q = w.randn(2).to(cuda), w.randn(4).to(cuda)
@@ -662,10 +661,15 @@ def test_refusals(bk, lib, cuda):
             make()
     # the C entry points, with a workspace that is missing or too small
     d = w.cache._batch(q, t.repeat(1, 200).contiguous(), l, None)      # sequences that may be long: their parts need space
-    need = lib.bikv_fp8_attend_workspace(w.cache._h, C.byref(d), 4)
+    need = lib.bikv_fp8_attend_workspace(w.cache._h, d, 4)
     assert need > 0
     for ws, size in ((None, need), (q.data_ptr(), need - 1), (q.data_ptr() + 4, need)):
-        assert lib.bikv_fp8_attend(w.cache._h, 1, C.byref(d), q.data_ptr(), 512, 128, 4, 1, 0.1, k.data_ptr(), 512, 128, None, ws, size, None) == _lib.EINVAL
-    d.max_pages = 1 << 40
-    d.page_table_stride = 1 << 40
-    assert lib.bikv_fp8_attend_workspace(w.cache._h, C.byref(d), 4) == _lib.ERANGE
+        assert lib.bikv_fp8_attend(w.cache._h, 1, d, q.data_ptr(), 512, 128, 4, 1, 0.1, k.data_ptr(), 512, 128, None, ws, size, None) == _lib.EINVAL
+    wide = struct.pack("=7q2i", t.data_ptr(), 1 << 40, 1 << 40, l.data_ptr(), 0, 2, 2, 0, 0)
+    assert lib.bikv_fp8_attend_workspace(w.cache._h, wide, 4) == _lib.ERANGE
+    for at, value in ((5, -1), (6, -2), (2, -1), (7, 2), (6, 3), (1, 0), (3, 0), (0, 0)):          # n_seqs, n_rows, max_pages, dtype, rows without starts, table stride, null arrays
+        f = list(struct.unpack("=7q2i", d))
+        f[at] = value
+        for call in (lambda b: lib.bikv_fp8_attend(w.cache._h, 1, b, q.data_ptr(), 512, 128, 4, 1, 0.1, k.data_ptr(), 512, 128, None, q.data_ptr(), need, None),
+                     lambda b: lib.bikv_fp8_append(w.cache._h, 1, b, k.data_ptr(), 256, 128, k.data_ptr(), 256, 128, None)):
+            assert call(struct.pack("=7q2i", *f)) == _lib.EINVAL, (at, value)
