@@ -45,8 +45,8 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {      // nearest, ties to even
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 __device__ __forceinline__ float half_of(uint32_t pair, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> (16 * i))); }
 template <int TYPE>
@@ -772,6 +772,7 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
+constexpr float kSlack = 4.f;           // p 2^kPShift vs 2^-r < 2^(4 + 8 + 1), in fp16's range
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -785,14 +786,16 @@ template <int D, int TYPE>
 __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArgs a) {
   constexpr int kKeys = kManyKeys;
   constexpr int kChunks = D / 8;                  // 16-byte pieces of a K row in LDS
-  constexpr int kVB = D / 16;                     // bytes of a V row per thread
-  constexpr int kLoads = D / 32;                  // 16-byte registers a thread brings per step
+  constexpr int kLoads = D / 64;                  // 16-byte pieces of K a thread brings per step
+  constexpr int kRowThreads = D / 4;              // threads that bring one row of V, four bytes each
   struct Meta {
     uint64_t off[kKeys];
-    float ks[kKeys], vs[kKeys];
+    float ks[kKeys], vs[kKeys];                   // times the softmax's scale and log2(e); times 2^(kPShift - r)
     int pos[kKeys];
-    int gone;
+    int gone, r;                                  // some key is nobody's; the largest exponent of V's scales up to here
+    float ks_in[kKeys], vs_in[kKeys];             // the scales as they are in the cache
   };
+  __shared__ uint32_t pid_in[2][kKeys];           // page ids of the keys to be looked up next, low and high words
   __shared__ int nan_at[D];                       // by place: the first key with a NaN in V that not every row sees
   __shared__ int spoilt;
   __shared__ u32x4 k_lds[2][kKeys * kChunks];
@@ -849,117 +852,115 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 
   const uint64_t kbase = (uint64_t)a.layer.k + h * D, vbase = (uint64_t)a.layer.v + h * D;
   const uint64_t trow = (uint64_t)(a.seq.table + b * a.seq.table_stride);
-  auto page_of = [&](int t) -> int64_t {
-    const int key = t * kKeys + lane;
-    if (key >= seen) return -1;
-    return gload<int64_t>(trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens));
+  // Wave 0 looks the keys of the steps ahead up, in three stages a step apart, through copies into LDS that hold no
+  // registers meanwhile: page ids; with them places and scales; with those what the step's metas say.
+  const uint32_t lds_pid = (uint32_t)uni((int)lds_address(pid_in));
+  auto copy_pages = [&](int t) {
+    int key = t * kKeys + lane;
+    key = key < seen ? key : seen - 1;
+    const uint64_t src = trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens);
+    copy4_to_lds(src, lds_pid);
+    copy4_to_lds(src + 4, lds_pid + 4 * kKeys);
   };
-  struct Key { uint64_t off; float ks, vs; int pos; };
-  auto look_up = [&](int t, int64_t pid) {
-    Key k = {0, 0.f, 0.f, kNoKey};
+  bool bad_page = false;
+  auto look_up = [&](int t, Meta& m) {
     const int key = t * kKeys + lane;
-    if (key < seen) {
-      if ((uint64_t)pid >= (uint64_t)a.layer.n_pages) {
-        raise_flag(a.status, ST_SLOT_PAGE);
-      } else {
-        const uint32_t in_page = (uint32_t)key - divide((uint32_t)key, a.layer.page_tokens) * (uint32_t)P;
-        k.off = (uint64_t)(pid * a.layer.page_stride) + (uint64_t)in_page * (uint64_t)a.layer.token_stride;
-        k.ks = gload<float>((uint64_t)a.layer.ks + 4 * h + (uint64_t)(pid * a.layer.scale_stride));
-        k.vs = gload<float>((uint64_t)a.layer.vs + 4 * h + (uint64_t)(pid * a.layer.scale_stride));
-        k.pos = key;
+    const uint64_t pid = pid_in[0][lane] | ((uint64_t)pid_in[1][lane] << 32);
+    const bool in = key < seen, ok = in && pid < (uint64_t)a.layer.n_pages;
+    bad_page |= in && !ok;
+    const int64_t page = ok ? (int64_t)pid : 0;                    // keys that are not there read the plane's first row
+    uint32_t in_page = (uint32_t)key - divide((uint32_t)key, a.layer.page_tokens) * (uint32_t)P;
+    in_page = ok ? in_page : 0;
+    m.off[lane] = (uint64_t)(page * a.layer.page_stride) + (uint64_t)in_page * (uint64_t)a.layer.token_stride;
+    m.pos[lane] = ok ? key : kNoKey;
+    copy4_to_lds((uint64_t)a.layer.ks + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.ks_in)));
+    copy4_to_lds((uint64_t)a.layer.vs + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.vs_in)));
+  };
+  int r_seen = -126;
+  auto put_meta = [&](Meta& m) {                                   // the scales' copies have arrived
+    const float vs = m.vs_in[lane];
+    const bool there = m.pos[lane] != kNoKey;
+    const int e = there ? scale_exponent(vs) : -126;
+    if (__ballot(e > r_seen)) {
+      int top = e;
+      for (int i = 32; i > 0; i >>= 1) {
+        const int y = __shfl_xor(top, i);
+        top = y > top ? y : top;
       }
+      r_seen = uni(top > r_seen ? top : r_seen);
     }
-    return k;
-  };
-  auto put_meta = [&](Meta& m, const Key& k) {
-    m.off[lane] = k.off;
-    m.ks[lane] = k.ks * a.scale_log2;
-    m.vs[lane] = k.vs;
-    m.pos[lane] = k.pos;
-    const bool gone = __ballot(k.pos == kNoKey) != 0;
-    if (lane == 0) m.gone = gone;
+    m.ks[lane] = m.ks_in[lane] * a.scale_log2;
+    m.vs[lane] = ldexpf(vs, kPShift - r_seen);
+    const bool gone = __ballot(!there) != 0;
+    if (lane == 0) {
+      m.gone = gone;
+      m.r = r_seen;
+    }
   };
 
-  // Bringing a step's bytes: waves 0 and 1 K, waves 2 and 3 V.
-  const int p = tid & 127;
-  const bool brings_v = wave >= 2;
-  u32x4 raw[kLoads];
+  // Bringing a step's bytes: of K a thread takes whole 16-byte pieces, of V four bytes of each of eight keys.
+  const int vg = tid / kRowThreads & 7, v_at = 4 * (tid % kRowThreads);
+  u32x4 raw_k[kLoads];
+  uint32_t raw_v[8];
+  auto v_key = [&](int c) { return 16 * (vg >> 1) + 8 * (c >> 2) + 4 * (vg & 1) + (c & 3); };
+  // Byte offsets in a buffer. A row's 16-byte pieces are XOR-ed with a number that all rows the same lane touches share, so
+  // every access is one base, XOR a constant, plus a constant. The bases go through an empty asm in every step:
+  // otherwise the compiler keeps each of the two dozen sums in a register of its own and spills them.
+  constexpr int kKRow = 2 * D, kVRow = 2 * kKeys;
+  auto swizzle_k = [](int key) { return kChunks == 16 ? key & 15 : (key >> 1) & 7; };
+  auto swizzle_v = [](int d) { return ((d >> 1) & 7) ^ ((d >> 4) & 1); };
+  auto opaque = [](uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto at_k = [&](int buf, uint32_t off) -> u32x4& { return *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(k_lds) + buf * (int)sizeof(k_lds[0]) + off); };
+  auto at_v = [&](int buf, uint32_t off) -> u32x4& { return *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(v_lds) + buf * (int)sizeof(v_lds[0]) + off); };
+  constexpr int kPieces = D / 16;
+  const uint32_t k_write = (tid / kPieces) * kKRow + 16 * ((2 * (tid % kPieces)) ^ swizzle_k(tid / kPieces));
+  const uint32_t v_write = v_at * kVRow + 16 * (vg ^ swizzle_v(v_at));
+  const uint32_t k_read = col * kKRow + 16 * (half ^ swizzle_k(col)), v_read = col * kVRow + 16 * (half ^ swizzle_v(col));
   auto bring = [&](const Meta& m) {
-    if (!brings_v) {
-      constexpr int kRowLanes = D / 16;             // threads that read one row
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int key = i * (128 / kRowLanes) + p / kRowLanes;
-        raw[i] = gload<u32x4>(kbase + m.off[key] + 16 * (p % kRowLanes));
-      }
-    } else {
-      const int g = p >> 4, at = (p & 15) * kVB;
+    for (int i = 0; i < kLoads; ++i) raw_k[i] = gload<u32x4>(kbase + m.off[i * (256 / kPieces) + tid / kPieces] + 16 * (tid % kPieces));
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int key = 16 * (g >> 1) + 8 * (c >> 2) + 4 * (g & 1) + (c & 3);
-        const uint64_t src = vbase + m.off[key] + at;
-        if constexpr (kVB == 8) {
-          const u32x2 y = gload<u32x2>(src);
-          raw[c / 2][2 * (c & 1)] = y[0];
-          raw[c / 2][2 * (c & 1) + 1] = y[1];
-        } else {
-          raw[c / 4][c & 3] = gload<uint32_t>(src);
-        }
-      }
-    }
+    for (int c = 0; c < 8; ++c) raw_v[c] = gload<uint32_t>(vbase + m.off[v_key(c)] + v_at);
   };
   auto put = [&](int t, int buf, const Meta& m) {
-    if (!brings_v) {
-      constexpr int kRowLanes = D / 16;
+    static_assert(256 / kPieces % 16 == 0, "the rows of a thread's pieces share their swizzle");
+    const uint32_t k_at = opaque(k_write);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int key = i * (128 / kRowLanes) + p / kRowLanes, c = 2 * (p % kRowLanes);
+    for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const u32x2 lo = widen4<TYPE>(raw[i][2 * e]), hi = widen4<TYPE>(raw[i][2 * e + 1]);
-          k_lds[buf][key * kChunks + ((c + e) ^ (key & (kChunks - 1)))] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-        }
+      for (int e = 0; e < 2; ++e) {
+        const u32x2 lo = widen4<TYPE>(raw_k[i][2 * e]), hi = widen4<TYPE>(raw_k[i][2 * e + 1]);
+        at_k(buf, (k_at ^ (16 * e)) + i * (256 / kPieces) * kKRow) = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
-    } else {
-      const int g = p >> 4, c16 = p & 15;
-      if ((t + 1) * kKeys > all || m.gone) {
-        // bytes of keys that nobody sees become zero, and so does a NaN: the rows that see its key get it at the end
-        uint32_t any = 0;
+    if ((t + 1) * kKeys > all || m.gone) {
+      // bytes of keys that nobody sees become zero, and so does a NaN: the rows that see its key get it at the end
+      uint32_t any = 0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int pos = m.pos[16 * (g >> 1) + 8 * (c >> 2) + 4 * (g & 1) + (c & 3)];
-#pragma unroll
-          for (int dw = 0; dw < kVB / 4; ++dw) {
-            const int r0 = kVB == 8 ? c / 2 : c / 4, r1 = kVB == 8 ? 2 * (c & 1) + dw : c & 3;
-            const uint32_t bytes = pos == kNoKey ? 0 : raw[r0][r1], bad = nan_bytes(bytes);
-            any |= bad;
-            raw[r0][r1] = bytes & ~bad;
-          }
-        }
-        if (__ballot(any != 0)) {
-          spoilt = 1;
-          if (m.pos[lane] != kNoKey) note_nans<D>(nan_at, vbase + m.off[lane], m.pos[lane]);
-        }
+      for (int c = 0; c < 8; ++c) {
+        const uint32_t bytes = m.pos[v_key(c)] == kNoKey ? 0 : raw_v[c], bad = nan_bytes(bytes);
+        any |= bad;
+        raw_v[c] = bytes & ~bad;
       }
+      if (__ballot(any != 0)) {
+        spoilt = 1;
+        if (m.pos[lane] != kNoKey) note_nans<D>(nan_at, vbase + m.off[lane], m.pos[lane]);
+      }
+    }
+    if (tid < 8 * kRowThreads) {
+      const uint32_t at = opaque(v_write);
+      u32x2 x8[8];
 #pragma unroll
-      for (int dw = 0; dw < kVB / 4; ++dw) {
-        u32x2 x8[8];
+      for (int c = 0; c < 8; ++c) x8[c] = widen4<1>(raw_v[c]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t bytes;
-          if constexpr (kVB == 8) bytes = raw[c / 2][2 * (c & 1) + dw];
-          else bytes = raw[c / 4][c & 3];
-          x8[c] = widen4<1>(bytes);
-        }
+      for (int pl = 0; pl < 4; ++pl) {
+        u32x4 f;
 #pragma unroll
-        for (int pl = 0; pl < 4; ++pl) {
-          u32x4 f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            f[c] = __builtin_amdgcn_perm(x8[2 * c + 1][pl / 2], x8[2 * c][pl / 2], pl & 1 ? 0x07060302u : 0x05040100u);
-          const int d = c16 * kVB + 4 * dw + pl;
-          v_lds[buf][d * 8 + (g ^ ((d >> 1) & 7))] = f;
-        }
+        for (int c = 0; c < 4; ++c)
+          f[c] = __builtin_amdgcn_perm(x8[2 * c + 1][pl / 2], x8[2 * c][pl / 2], pl & 1 ? 0x07060302u : 0x05040100u);
+        at_v(buf, (at ^ (16 * (pl >> 1))) + pl * kVRow) = f;
       }
     }
   };
@@ -971,124 +972,174 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float m_run = kMinusInf, l_run = 0.f;
   int r_exp = -126;
+  auto scale_sums = [&](float by) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[i][c] *= by;
+  };
 
   auto compute = [&](int t, int buf, const Meta& meta) {
-    {
-      const float vs = meta.vs[lane];
-      const int e = meta.pos[lane] == kNoKey ? -126 : scale_exponent(vs);
-      if (__ballot(e > r_exp)) {
-        int top = e;
-        for (int k = 32; k > 0; k >>= 1) {
-          const int y = __shfl_xor(top, k);
-          top = y > top ? y : top;
-        }
-        top = uni(top);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int c = 0; c < 16; ++c) o[i][c] = ldexpf(o[i][c], r_exp - top);
-        r_exp = top;
-      }
-    }
-    const bool edge = (t + 1) * kKeys > wave_all || meta.gone;
-    f32x16 s[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-      const int key = 32 * kb + col;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        s[kb] = mfma32<TYPE>(k_lds[buf][key * kChunks + ((2 * j + half) ^ (key & (kChunks - 1)))], q[j], s[kb]);
-    }
-    // the lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4
-    float top = kMinusInf;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 ks = *reinterpret_cast<const f32x4*>(&meta.ks[32 * kb + 8 * j + 4 * half]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float z = s[kb][4 * j + c] * ks[c];
-          if (edge && meta.pos[32 * kb + 8 * j + 4 * half + c] >= limit) z = kMinusInf;
-          s[kb][4 * j + c] = z;
-          top = fmaxf(top, z);
-        }
-      }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__ballot(top > m_run)) {
-      const float now = fmaxf(m_run, top);
-      const float grow = now == kMinusInf ? 1.f : exp2_fast(m_run - now);
-      m_run = now;
-      l_run *= grow;
+    const int r = uni(meta.r);
+    if (r != r_exp) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int c = 0; c < 16; ++c) o[i][c] *= grow;
+        for (int c = 0; c < 16; ++c) o[i][c] = ldexpf(o[i][c], r_exp - r);
+      r_exp = r;
     }
-    const float from = m_run == kMinusInf ? 0.f : m_run;
+    const bool edge = (t + 1) * kKeys > wave_all || uni(meta.gone);
+    // Operands are read from LDS half a step ahead of the products that use them, each into the registers of the
+    // operand just used; left alone, the compiler reads each one right before its product and waits for it.
+    f32x16 s[2];
+    u32x4 kf[D / 16];
+    f32x4 ks[2][4];
+    const uint32_t k_at = opaque(k_read), v_at = opaque(v_read);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) kf[j] = at_k(buf, k_at ^ (32 * j));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      s[0] = mfma32<TYPE>(kf[j], q[j], s[0]);
+      kf[j] = at_k(buf, (k_at ^ (32 * j)) + 32 * kKRow);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ks[i / 4][i & 3] = *reinterpret_cast<const f32x4*>(&meta.ks[32 * (i / 4) + 8 * (i & 3) + 4 * half]);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    // The lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4. z is taken against the row's last reference m, which is
+    // moved only when some z exceeds it by kSlack: p may then be up to 2^kSlack, which fp16 has room for, and most steps
+    // rescale nothing and reduce nothing across lanes.
+    float from = m_run == kMinusInf ? 0.f : m_run, top = kMinusInf;
+    uint32_t hidden = 0;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        u32x4 pf;
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key0 = 32 * kb + 16 * s2 + 8 * j + 4 * half;
-          const f32x4 vs = *reinterpret_cast<const f32x4*>(&meta.vs[key0]);
-          float f[4];
+        for (int c = 0; c < 4; ++c) s[kb][4 * j + c] = fmaf(s[kb][4 * j + c], ks[kb][j][c], -from);
+    if (edge) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float e = exp2_fast(s[kb][8 * s2 + 4 * j + c] - from);
-            l_run += e;
-            f[c] = e * ldexpf(vs[c], kPShift - r_exp);
-            if (edge && meta.pos[key0 + c] >= limit) f[c] = 0.f;
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (meta.pos[32 * kb + 8 * (i / 4) + 4 * half + (i & 3)] >= limit) {
+            s[kb][i] = kMinusInf;
+            hidden |= 1u << (16 * kb + i);
           }
-          pf[2 * j] = pack_f16(f[0], f[1]);
-          pf[2 * j + 1] = pack_f16(f[2], f[3]);
-        }
-        const int g = 2 * (2 * kb + s2) + half;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    if (__ballot(top > kSlack || (m_run == kMinusInf && top > kMinusInf))) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // a row moves if it has to or has no reference yet (the halves of a row agree: top is the row's)
+      const bool move = top > kSlack || (m_run == kMinusInf && top > kMinusInf);
+      const float by = move ? top : 0.f;
+      const float grow = m_run == kMinusInf ? 0.f : exp2_fast(-by);
+      if (move) m_run = from + by;
+      l_run *= grow;
+      scale_sums(grow);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] -= by;
+    }
+    f32x4 vs[2][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vs[i / 4][i & 3] = *reinterpret_cast<const f32x4*>(&meta.vs[32 * (i / 4) + 8 * (i & 3) + 4 * half]);
+    u32x4 vf[2][D / 32];
+    auto read_v = [&](int kb, int s2, int dt) { vf[s2][dt] = at_v(buf, (v_at ^ (32 * (2 * kb + s2))) + 32 * dt * kVRow); };
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) read_v(0, s2, dt);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_fast(s[kb][i]);
+        l_run += e;
+        s[kb][i] = e * vs[kb][i / 4][i & 3];
+      }
+    if (edge) {                                    // 0 times a scale that is not finite
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if ((hidden >> (16 * kb + i)) & 1u) s[kb][i] = 0.f;
+    }
+    u32x4 pf[2][2], pf_low[2][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t y = pack_f16(s[kb][i], s[kb][i + 1]);
+        pf[kb][i / 8][(i & 7) / 2] = y;
+        if constexpr (TYPE == 1) pf_low[kb][i / 8][(i & 7) / 2] = pack_f16(s[kb][i] - half_of(y, 0), s[kb][i + 1] - half_of(y, 1));
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
-          const int d = 32 * dt + col;
-          const u32x4 f = v_lds[buf][d * 8 + (g ^ ((d >> 1) & 7))];
-          o[dt] = mfma32<1>(f, pf, o[dt]);
+          o[dt] = mfma32<1>(vf[s2][dt], pf[kb][s2], o[dt]);
+          if constexpr (TYPE == 1) o[dt] = mfma32<1>(vf[s2][dt], pf_low[kb][s2], o[dt]);
+          if (kb == 0) {
+            read_v(1, s2, dt);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
-      }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   if (t0 < t1) {
     // Step t's bytes are brought while step t - 1 is computed, its keys' places one step earlier.
-    Key next = {0, 0.f, 0.f, kNoKey};
-    int64_t pid = -1;
     if (wave == 0) {
-      put_meta(metas[0], look_up(t0, page_of(t0)));
-      if (t0 + 1 < t1) put_meta(metas[1], look_up(t0 + 1, page_of(t0 + 1)));
-      if (t0 + 2 < t1) pid = page_of(t0 + 2);
+      for (int i = 0; i < 2; ++i) {
+        copy_pages(t0 + i);
+        wait_vmem<0>();
+        look_up(t0 + i, metas[i]);
+        wait_vmem<0>();
+        put_meta(metas[i]);
+      }
+      copy_pages(t0 + 2);
     }
     for (int d = tid; d < D; d += 256) nan_at[d] = kNoKey;
     if (tid == 0) spoilt = 0;
-    __syncthreads();
+    lds_barrier();
     bring(metas[0]);
     put(t0, 0, metas[0]);
-    __syncthreads();
+    lds_barrier();
     int mi = 0;
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
       const int m1 = mi == 2 ? 0 : mi + 1, m2 = m1 == 2 ? 0 : m1 + 1;
-      if (t + 1 < t1) bring(metas[m1]);
-      if (wave == 0 && t + 2 < t1) {
-        next = look_up(t + 2, pid);
-        if (t + 3 < t1) pid = page_of(t + 3);
+      if (wave == 0) {
+        wait_vmem<0>();                            // the page ids of t + 2, asked for a step ago
+        look_up(t + 2, metas[m2]);
+        copy_pages(t + 3);
       }
+      bring(metas[m1]);
       if (t * kKeys < wave_seen) compute(t, buf, metas[mi]);
       if (t + 1 < t1) put(t + 1, buf ^ 1, metas[m1]);
-      if (wave == 0 && t + 2 < t1) put_meta(metas[m2], next);
-      __syncthreads();
+      if (wave == 0) {
+        wait_vmem<0>();                            // here anyway: older than the bytes that put() has waited for
+        put_meta(metas[m2]);
+      }
+      lds_barrier();
       mi = m1;
     }
-    if (spoilt)
+    if (bad_page) raise_flag(a.status, ST_SLOT_PAGE);
+  if (spoilt)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
