@@ -790,17 +790,16 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   constexpr int kRowThreads = D / 4;              // threads that bring one row of V, four bytes each
   struct Meta {
     uint64_t off[kKeys];
-    float ks[kKeys], vs[kKeys];                   // times the softmax's scale and log2(e); times 2^(kPShift - r)
+    float ks[kKeys], vs[kKeys];                   // as they are in the cache; then times the softmax's scale and log2(e), and times 2^(kPShift - r)
     int pos[kKeys];
-    int gone, r;                                  // some key is nobody's; the largest exponent of V's scales up to here
-    float ks_in[kKeys], vs_in[kKeys];             // the scales as they are in the cache
+    int gone, e, r;                               // some key is nobody's; the largest exponent of V's scales here; and up to here
   };
-  __shared__ uint32_t pid_in[2][kKeys];           // page ids of the keys to be looked up next, low and high words
+  __shared__ uint32_t pids_in[4][2][kKeys];       // page ids of the keys to be looked up next, low and high words
   __shared__ int nan_at[D];                       // by place: the first key with a NaN in V that not every row sees
   __shared__ int spoilt;
   __shared__ u32x4 k_lds[2][kKeys * kChunks];
   __shared__ u32x4 v_lds[2][D * 8];
-  __shared__ Meta metas[3];
+  __shared__ Meta metas[8];
   const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63;
   const int half = lane >> 5, col = lane & 31;
   const uint32_t H = (uint32_t)a.layer.heads;
@@ -832,40 +831,53 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   const int per = (steps + a.slots - 1) / a.slots;
   const int t0 = part * per, t1 = t0 + per < steps ? t0 + per : steps;
 
+  auto opaque = [](uint32_t x) {                   // keeps the compiler from holding in registers what it could work out again
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   // the wave's rows: row0 + 32 wave + col
-  const int r = 32 * wave + col;
-  const bool live = r < rows;
-  const uint32_t row = (uint32_t)(row0 + (live ? r : 0));
-  const uint32_t tok = divide(row, a.group);
-  const int head = h * G + (int)(row - tok * G);
-  const int limit = sees((int)row);
+  struct Row { int r; bool live; uint32_t tok; int head; };
+  auto my_row = [&](int c) {
+    Row y;
+    y.r = 32 * wave + c;
+    y.live = y.r < rows;
+    const uint32_t row = (uint32_t)(row0 + (y.live ? y.r : 0));
+    y.tok = divide(row, a.group);
+    y.head = h * G + (int)(row - y.tok * G);
+    return y;
+  };
+  const int limit = sees(row0 + (32 * wave + col < rows ? 32 * wave + col : 0));
   const int wave_last = 32 * wave + 31 < rows ? 32 * wave + 31 : rows - 1;
   const int wave_seen = uni(32 * wave < rows ? sees(row0 + wave_last) : 0);
   const int wave_all = uni(32 * wave < rows ? sees(row0 + 32 * wave) : 0);
   const int all = uni(sees(row0));                 // keys that every row of the tile sees
   u32x4 q[D / 16];
   {
-    const uint64_t src = (uint64_t)a.q + 2 * ((seq.first + tok) * a.q_row + head * a.q_head);
+    const Row me = my_row(col);
+    const uint64_t src = (uint64_t)a.q + 2 * ((seq.first + me.tok) * a.q_row + me.head * a.q_head);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) q[j] = gload<u32x4>(src + 2 * (16 * j + 8 * half));
   }
 
   const uint64_t kbase = (uint64_t)a.layer.k + h * D, vbase = (uint64_t)a.layer.v + h * D;
   const uint64_t trow = (uint64_t)(a.seq.table + b * a.seq.table_stride);
-  // Wave 0 looks the keys of the steps ahead up, in three stages a step apart, through copies into LDS that hold no
-  // registers meanwhile: page ids; with them places and scales; with those what the step's metas say.
+  // The keys of four steps are looked up at a time, a step's by each wave, in stages a step or more apart and through
+  // copies into LDS that hold no registers meanwhile: page ids; with them places and scales; with the scales
+  // their largest exponent; with those of all four what is left of the steps' metas. Step t's is metas[(t - t0) & 7].
+  uint32_t (*pid_in)[kKeys] = pids_in[wave];
   const uint32_t lds_pid = (uint32_t)uni((int)lds_address(pid_in));
-  auto copy_pages = [&](int t) {
+  auto table_at = [&](int t) {
     int key = t * kKeys + lane;
     key = key < seen ? key : seen - 1;
-    const uint64_t src = trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens);
-    copy4_to_lds(src, lds_pid);
-    copy4_to_lds(src + 4, lds_pid + 4 * kKeys);
+    return trow + 8 * (uint64_t)divide((uint32_t)key, a.layer.page_tokens);
+  };
+  auto copy_pages = [&](int t) {
+    copy4_to_lds(table_at(t), lds_pid);
+    copy4_to_lds(table_at(t) + 4, lds_pid + 4 * kKeys);
   };
   bool bad_page = false;
-  auto look_up = [&](int t, Meta& m) {
+  auto look_up = [&](int t, uint64_t pid, Meta& m) {
     const int key = t * kKeys + lane;
-    const uint64_t pid = pid_in[0][lane] | ((uint64_t)pid_in[1][lane] << 32);
     const bool in = key < seen, ok = in && pid < (uint64_t)a.layer.n_pages;
     bad_page |= in && !ok;
     const int64_t page = ok ? (int64_t)pid : 0;                    // keys that are not there read the plane's first row
@@ -873,29 +885,29 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     in_page = ok ? in_page : 0;
     m.off[lane] = (uint64_t)(page * a.layer.page_stride) + (uint64_t)in_page * (uint64_t)a.layer.token_stride;
     m.pos[lane] = ok ? key : kNoKey;
-    copy4_to_lds((uint64_t)a.layer.ks + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.ks_in)));
-    copy4_to_lds((uint64_t)a.layer.vs + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.vs_in)));
+    const bool gone = __ballot(!ok) != 0;
+    if (lane == 0) m.gone = gone;
+    copy4_to_lds((uint64_t)a.layer.ks + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.ks)));
+    copy4_to_lds((uint64_t)a.layer.vs + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.vs)));
+  };
+  auto find_exponent = [&](Meta& m) {
+    int e = m.pos[lane] != kNoKey ? scale_exponent(m.vs[lane]) : -126;
+    for (int i = 32; i > 0; i >>= 1) {
+      const int y = __shfl_xor(e, i);
+      e = y > e ? y : e;
+    }
+    if (lane == 0) m.e = e;
   };
   int r_seen = -126;
-  auto put_meta = [&](Meta& m) {                                   // the scales' copies have arrived
-    const float vs = m.vs_in[lane];
-    const bool there = m.pos[lane] != kNoKey;
-    const int e = there ? scale_exponent(vs) : -126;
-    if (__ballot(e > r_seen)) {
-      int top = e;
-      for (int i = 32; i > 0; i >>= 1) {
-        const int y = __shfl_xor(top, i);
-        top = y > top ? y : top;
-      }
-      r_seen = uni(top > r_seen ? top : r_seen);
+  auto finish = [&](int first, Meta& m) {                          // first: the ring's index of the four steps' first
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = uni(metas[first + i].e);
+      r_seen = e > r_seen ? e : r_seen;
     }
-    m.ks[lane] = m.ks_in[lane] * a.scale_log2;
-    m.vs[lane] = ldexpf(vs, kPShift - r_seen);
-    const bool gone = __ballot(!there) != 0;
-    if (lane == 0) {
-      m.gone = gone;
-      m.r = r_seen;
-    }
+    m.ks[lane] *= a.scale_log2;
+    m.vs[lane] = ldexpf(m.vs[lane], kPShift - r_seen);
+    if (lane == 0) m.r = r_seen;
   };
 
   // Bringing a step's bytes: of K a thread takes whole 16-byte pieces, of V four bytes of each of eight keys.
@@ -909,10 +921,6 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   constexpr int kKRow = 2 * D, kVRow = 2 * kKeys;
   auto swizzle_k = [](int key) { return kChunks == 16 ? key & 15 : (key >> 1) & 7; };
   auto swizzle_v = [](int d) { return ((d >> 1) & 7) ^ ((d >> 4) & 1); };
-  auto opaque = [](uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-  };
   auto at_k = [&](int buf, uint32_t off) -> u32x4& { return *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(k_lds) + buf * (int)sizeof(k_lds[0]) + off); };
   auto at_v = [&](int buf, uint32_t off) -> u32x4& { return *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(v_lds) + buf * (int)sizeof(v_lds[0]) + off); };
   constexpr int kPieces = D / 16;
@@ -994,6 +1002,10 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     f32x16 s[2];
     u32x4 kf[D / 16];
     f32x4 ks[2][4];
+    auto read_ks = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ks[kb][i] = *reinterpret_cast<const f32x4*>(&meta.ks[32 * kb + 8 * i + 4 * half]);
+    };
     const uint32_t k_at = opaque(k_read), v_at = opaque(v_read);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) kf[j] = at_k(buf, k_at ^ (32 * j));
@@ -1006,10 +1018,11 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       kf[j] = at_k(buf, (k_at ^ (32 * j)) + 32 * kKRow);
       __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ks[i / 4][i & 3] = *reinterpret_cast<const f32x4*>(&meta.ks[32 * (i / 4) + 8 * (i & 3) + 4 * half]);
+    read_ks(0);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    read_ks(1);
     __builtin_amdgcn_sched_barrier(0);
     // The lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4. z is taken against the row's last reference m, which is
     // moved only when some z exceeds it by kSlack: p may then be up to 2^kSlack, which fp16 has room for, and most steps
@@ -1102,42 +1115,37 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   };
 
   if (t0 < t1) {
-    // Step t's bytes are brought while step t - 1 is computed, its keys' places one step earlier.
-    if (wave == 0) {
-      for (int i = 0; i < 2; ++i) {
-        copy_pages(t0 + i);
-        wait_vmem<0>();
-        look_up(t0 + i, metas[i]);
-        wait_vmem<0>();
-        put_meta(metas[i]);
-      }
-      copy_pages(t0 + 2);
-    }
+    // Step t's bytes are brought while step t - 1 is computed.
+    look_up(t0 + wave, gload<uint64_t>(table_at(t0 + wave)), metas[wave]);
+    copy_pages(t0 + 4 + wave);
     for (int d = tid; d < D; d += 256) nan_at[d] = kNoKey;
     if (tid == 0) spoilt = 0;
     lds_barrier();
     bring(metas[0]);
+    wait_vmem<0>();
+    find_exponent(metas[wave]);
+    lds_barrier();
+    finish(0, metas[wave]);
     put(t0, 0, metas[0]);
     lds_barrier();
-    int mi = 0;
     for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      const int m1 = mi == 2 ? 0 : mi + 1, m2 = m1 == 2 ? 0 : m1 + 1;
-      if (wave == 0) {
-        wait_vmem<0>();                            // the page ids of t + 2, asked for a step ago
-        look_up(t + 2, metas[m2]);
-        copy_pages(t + 3);
+      const int i = t - t0, ahead = (i & 4) ^ 4;   // ahead: where the ring has the next four steps
+      if ((i & 3) == 0) {
+        wait_vmem<0>();                            // the page ids, asked for four steps ago
+        look_up(t + 4 + wave, pid_in[0][lane] | ((uint64_t)pid_in[1][lane] << 32), metas[ahead + wave]);
+        copy_pages(t + 8 + wave);
+      } else if ((i & 3) == 1) {
+        wait_vmem<0>();                            // the scales, asked for a step ago
+        find_exponent(metas[ahead + wave]);
+      } else if ((i & 3) == 3) {
+        finish(ahead, metas[ahead + wave]);
       }
-      bring(metas[m1]);
-      if (t * kKeys < wave_seen) compute(t, buf, metas[mi]);
-      if (t + 1 < t1) put(t + 1, buf ^ 1, metas[m1]);
-      if (wave == 0) {
-        wait_vmem<0>();                            // here anyway: older than the bytes that put() has waited for
-        put_meta(metas[m2]);
-      }
+      bring(metas[(i + 1) & 7]);
+      if (t * kKeys < wave_seen) compute(t, i & 1, metas[i & 7]);
+      if (t + 1 < t1) put(t + 1, (i & 1) ^ 1, metas[(i + 1) & 7]);
       lds_barrier();
-      mi = m1;
     }
+    wait_vmem<0>();                                // no copy into LDS outlives the workgroup
     if (bad_page) raise_flag(a.status, ST_SLOT_PAGE);
   if (spoilt)
 #pragma unroll
@@ -1149,7 +1157,10 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 
   l_run += __shfl_xor(l_run, 32);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-  if (!live) return;
+  const Row me = my_row((int)opaque((uint32_t)col));
+  const uint32_t tok = me.tok;
+  const int head = me.head, r = me.r, by_half = (int)opaque((uint32_t)half);
+  if (!me.live) return;
   if (a.slots == 1) {
     const uint64_t dst = (uint64_t)a.out + 2 * ((seq.first + tok) * a.o_row + head * a.o_head);
 #pragma unroll
@@ -1159,9 +1170,9 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         float y[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, r_exp - kPShift);
-        gstore<u32x2>(dst + 2 * (32 * i + 8 * j + 4 * half), u32x2{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3])});
+        gstore<u32x2>(dst + 2 * (32 * i + 8 * j + 4 * by_half), u32x2{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3])});
       }
-    if (a.lse && half == 0)
+    if (a.lse && by_half == 0)
       a.lse[(seq.first + tok) * (int64_t)(H * G) + head] = l_run == 0.f ? kMinusInf : (m_run + __log2f(l_run)) * 0.69314718055994530942f;
   } else {
     const int64_t at = ((slot * H + h) * a.slots + part) * kManyRows + r;
@@ -1174,24 +1185,25 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
           f32x4 y;
 #pragma unroll
           for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, r_exp - kPShift);
-          gstore<f32x4>(dst + 4 * (32 * i + 8 * j + 4 * half), y);
+          gstore<f32x4>(dst + 4 * (32 * i + 8 * j + 4 * by_half), y);
         }
     }
-    if (half == 0) {
+    if (by_half == 0) {
       a.part_ml[2 * at] = m_run;
       a.part_ml[2 * at + 1] = l_run;
     }
   }
 }
 
-// A wave per row: joins the parts of a tile's keys.
+// Joins the parts of a tile's keys: D/4 threads a row, each with four places over all parts, of which there are few.
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) {
-  const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int kRows = 256 / (D / 4);            // rows of a workgroup
+  const int lane = threadIdx.x & 63;
   const int H = a.layer.heads, G = (int)a.group.d;
   const uint32_t id = blockIdx.x;
-  const int r = (int)(id % (kManyRows / 4)) * 4 + wave;
-  const uint32_t rest = id / (kManyRows / 4);
+  const int r = (int)(id % (kManyRows / kRows)) * kRows + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
+  const uint32_t rest = id / (kManyRows / kRows);
   const int h = (int)(rest % (uint32_t)H);
   const int64_t slot = rest / (uint32_t)H;
   const int64_t b = find_seq(a.seq.n_seqs, slot, lane, [&](int64_t i) { return first_tile<kManyRows>(a, i); });
@@ -1200,7 +1212,25 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
   if (!seq.ok || tile < 0 || tile * kManyRows + r >= (int64_t)seq.n * G) return;
   const uint32_t row = (uint32_t)(tile * kManyRows + r), tok = divide(row, a.group);
   auto at = [&](int i) { return ((slot * H + h) * a.slots + i) * kManyRows + r; };
-  join_row<D, TYPE>(a, lane, a.slots, at, seq.first + tok, h * G + (int)(row - tok * G), H * G);
+  float top = kMinusInf;
+  for (int i = 0; i < a.slots; ++i) top = fmaxf(top, a.part_ml[2 * at(i)]);
+  const float from = top == kMinusInf ? 0.f : top;
+  f32x4 o = {0, 0, 0, 0};
+  float sum = 0.f;
+  for (int i = 0; i < a.slots; ++i) {
+    float w = a.part_ml[2 * at(i) + 1];
+    if (w == 0.f) continue;                       // saw no key: what it holds was never written
+    w *= exp2_fast(a.part_ml[2 * at(i)] - from);
+    const f32x4 y = gload<f32x4>((uint64_t)(a.part_o + at(i) * D + d));
+    sum += w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += w * y[c];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int head = h * G + (int)(row - tok * G);
+  gstore<u32x2>((uint64_t)a.out + 2 * ((seq.first + tok) * a.o_row + head * a.o_head + d),
+                u32x2{narrow<TYPE>(o[0] * inv, o[1] * inv), narrow<TYPE>(o[2] * inv, o[3] * inv)});
+  if (a.lse && d == 0) a.lse[(seq.first + tok) * (int64_t)(H * G) + head] = sum == 0.f ? kMinusInf : (top + __log2f(sum)) * 0.69314718055994530942f;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1231,7 +1261,7 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
     p.tiles = all / kManyRows + n_seqs;
-    int64_t parts = 512 / (p.tiles * heads);
+    int64_t parts = (512 + p.tiles * heads / 2) / (p.tiles * heads);       // two workgroups to a CU
     const int64_t steps = (max_len + kManyKeys - 1) / kManyKeys;
     if (parts > steps / 4) parts = steps / 4;
     p.slots = (int32_t)(parts < 1 ? 1 : parts);
@@ -1258,7 +1288,7 @@ static hipError_t launch_form(const AttendPlan& p, const AttendArgs& a, hipStrea
   }
   hipLaunchKernelGGL((fp8_attend_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * p.slots)), dim3(256), 0, s, a);
   if (p.slots > 1)
-    hipLaunchKernelGGL((fp8_join_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * (kManyRows / 4))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((fp8_join_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * (kManyRows * D / 1024))), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
