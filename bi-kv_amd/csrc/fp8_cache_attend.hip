@@ -1018,23 +1018,31 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       kf[j] = at_k(buf, (k_at ^ (32 * j)) + 32 * kKRow);
       __builtin_amdgcn_sched_barrier(0);
     }
-    read_ks(0);
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
-    __builtin_amdgcn_sched_barrier(0);
-    read_ks(1);
-    __builtin_amdgcn_sched_barrier(0);
     // The lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4. z is taken against the row's last reference m, which is
     // moved only when some z exceeds it by kSlack: p may then be up to 2^kSlack, which fp16 has room for, and most steps
     // rescale nothing and reduce nothing across lanes.
-    float from = m_run == kMinusInf ? 0.f : m_run, top = kMinusInf;
+    const float from = m_run == kMinusInf ? 0.f : m_run;
+    float top = kMinusInf;
+    auto take_z = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = fmaf(s[kb][i], ks[kb][i / 4][i & 3], -from);
+    };
+    read_ks(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // the first half's z stand between the second half's products
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
+    take_z(0);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      if (j >= D / 32) __builtin_amdgcn_sched_group_barrier(0x2, 512 / D, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    read_ks(1);
+    __builtin_amdgcn_sched_barrier(0);
+    take_z(1);
     uint32_t hidden = 0;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[kb][4 * j + c] = fmaf(s[kb][4 * j + c], ks[kb][j][c], -from);
     if (edge) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -1051,7 +1059,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
     if (__ballot(top > kSlack || (m_run == kMinusInf && top > kMinusInf))) {
       top = fmaxf(top, __shfl_xor(top, 32));
-      // a row moves if it has to or has no reference yet (the halves of a row agree: top is the row's)
+      // a row moves if it has to or has no reference yet; its two lanes agree
       const bool move = top > kSlack || (m_run == kMinusInf && top > kMinusInf);
       const float by = move ? top : 0.f;
       const float grow = m_run == kMinusInf ? 0.f : exp2_fast(-by);
@@ -1064,53 +1072,71 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         for (int i = 0; i < 16; ++i) s[kb][i] -= by;
     }
     f32x4 vs[2][4];
+    auto read_vs = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vs[i / 4][i & 3] = *reinterpret_cast<const f32x4*>(&meta.vs[32 * (i / 4) + 8 * (i & 3) + 4 * half]);
+      for (int i = 0; i < 4; ++i) vs[kb][i] = *reinterpret_cast<const f32x4*>(&meta.vs[32 * kb + 8 * i + 4 * half]);
+    };
     u32x4 vf[2][D / 32];
     auto read_v = [&](int kb, int s2, int dt) { vf[s2][dt] = at_v(buf, (v_at ^ (32 * (2 * kb + s2))) + 32 * dt * kVRow); };
+    read_vs(0);
+    read_vs(1);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) read_v(0, s2, dt);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    u32x4 pf[2][2], pf_low[2][2];
+    auto weights = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e = exp2_fast(s[kb][i]);
         l_run += e;
         s[kb][i] = e * vs[kb][i / 4][i & 3];
       }
-    if (edge) {                                    // 0 times a scale that is not finite
+    };
+    auto blank = [&](int kb) {                     // 0 times a scale that is not finite
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if ((hidden >> (16 * kb + i)) & 1u) s[kb][i] = 0.f;
-    }
-    u32x4 pf[2][2], pf_low[2][2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int i = 0; i < 16; ++i)
+        if ((hidden >> (16 * kb + i)) & 1u) s[kb][i] = 0.f;
+    };
+    auto pack = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const uint32_t y = pack_f16(s[kb][i], s[kb][i + 1]);
         pf[kb][i / 8][(i & 7) / 2] = y;
         if constexpr (TYPE == 1) pf_low[kb][i / 8][(i & 7) / 2] = pack_f16(s[kb][i] - half_of(y, 0), s[kb][i + 1] - half_of(y, 1));
       }
+    };
+    auto gather = [&](int kb, int s2, int dt) {
+      o[dt] = mfma32<1>(vf[s2][dt], pf[kb][s2], o[dt]);
+      if constexpr (TYPE == 1) o[dt] = mfma32<1>(vf[s2][dt], pf_low[kb][s2], o[dt]);
+    };
+    weights(0);
+    if (edge) blank(0);
+    pack(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // the second half's exponentials stand between the first half's products
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        gather(0, s2, dt);
+        read_v(1, s2, dt);
+      }
+    weights(1);
+#pragma unroll
+    for (int i = 0; i < 2 * (D / 32); ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, TYPE == 1 ? 2 : 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 768 / D, 0);
+    }
+    if (edge) blank(1);
+    pack(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          o[dt] = mfma32<1>(vf[s2][dt], pf[kb][s2], o[dt]);
-          if constexpr (TYPE == 1) o[dt] = mfma32<1>(vf[s2][dt], pf_low[kb][s2], o[dt]);
-          if (kb == 0) {
-            read_v(1, s2, dt);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
+      for (int dt = 0; dt < D / 32; ++dt) gather(1, s2, dt);
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -1147,7 +1173,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     }
     wait_vmem<0>();                                // no copy into LDS outlives the workgroup
     if (bad_page) raise_flag(a.status, ST_SLOT_PAGE);
-  if (spoilt)
+    if (spoilt)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
