@@ -59,11 +59,30 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+typedef __attribute__((ext_vector_type(2))) short s16x2;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+// Four values, two to a word as they were read, divided by a power of two and rounded to the nearest e4m3.
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack4_scaled(uint32_t ab, uint32_t cd, float s) {
+  s16x2 w{0, 0};
+  if constexpr (TYPE == 0) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, ab), s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, cd), s, true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, ab), s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, cd), s, true);
+  }
+  return __builtin_bit_cast(uint32_t, w);
+}
+
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRows = 64 / kLanesPerRow;    // rows a wave reads with one instruction
-  constexpr int kVecs = 8;
+  constexpr int kVecs = 8, kOld = 4;
   constexpr int kChunk = kRows * kVecs;       // rows held in registers
   const int lane = threadIdx.x & 63;
   const uint32_t w = blockIdx.x * 4 + uni(threadIdx.x >> 6);    // below 2^31: the host sees to it
@@ -98,11 +117,7 @@ __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
   const int start = s.len - s.n;
   const int64_t page_no = (int64_t)divide((uint32_t)start, a.layer.page_tokens) + j;
   if (j < 0 || s.n == 0 || page_no * P >= s.len) return;
-  const int64_t pid = a.seq.table[b * a.seq.table_stride + page_no];
-  if ((uint64_t)pid >= (uint64_t)a.layer.n_pages) {
-    if (lane == 0) raise_flag(a.status, ST_SLOT_PAGE);
-    return;
-  }
+  const int64_t pid = a.seq.table[b * a.seq.table_stride + page_no];      // not looked at before the new values are on their way
   const int base = (int)(page_no * P);
   const int r0 = start > base ? start - base : 0;
   const int r1 = s.len - base < P ? s.len - base : P;
@@ -112,11 +127,9 @@ __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
   const int d = (lane % kLanesPerRow) * 8;
   const int64_t row = kv ? a.v_row : a.k_row, head = kv ? a.v_head : a.k_head;
   const uint64_t src = (uint64_t)(kv ? a.v : a.k) + 2 * ((s.first + (base + r0 - start)) * row + h * head + d);
-  const uint64_t page = (uint64_t)(kv ? a.layer.v : a.layer.k) + (uint64_t)(pid * a.layer.page_stride) + h * D + d;
-  const uint64_t scale_at = (uint64_t)(kv ? a.layer.vs : a.layer.ks) + (uint64_t)(pid * a.layer.scale_stride) + 4 * h;
-
   u32x4 x[kVecs];
-  float amax = 0.f;
+  constexpr uint32_t kInf = TYPE == 0 ? 0x7f80u : 0x7c00u;
+  u16x2 top{0, 0};                            // the largest |x| by its bits, which order like the values; two lanes of 16 bits
   auto load = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -125,38 +138,86 @@ __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
       if (r < n) x[i] = gload<u32x4>(src + 2 * (uint64_t)(r * row));
     }
   };
+  load(0);
+  __builtin_amdgcn_sched_barrier(0);
+  if ((uint64_t)pid >= (uint64_t)a.layer.n_pages) {
+    if (lane == 0) raise_flag(a.status, ST_SLOT_PAGE);
+    return;
+  }
+  const uint64_t page = (uint64_t)(kv ? a.layer.v : a.layer.k) + (uint64_t)(pid * a.layer.page_stride) + h * D + d;
+  const uint64_t scale_at = (uint64_t)(kv ? a.layer.vs : a.layer.ks) + (uint64_t)(pid * a.layer.scale_stride) + 4 * h;
+
   const float s_old = r0 > 0 ? gload<float>(scale_at) : 0.f;
   const int chunks = (n + kChunk - 1) / kChunk;
   for (int c = 0; c < chunks; ++c) {
-    load(c * kChunk);
+    if (c > 0) load(c * kChunk);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float lo = fabsf(widen<TYPE>(x[i][e] & 0xffffu)), hi = fabsf(widen<TYPE>(x[i][e] >> 16));
-        if (finite_bits(lo)) amax = fmaxf(amax, lo);
-        if (finite_bits(hi)) amax = fmaxf(amax, hi);
-      }
+      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x[i][e] & 0x7fff7fffu));
   }
-  for (int m = 32; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+  uint32_t bits = top[0] > top[1] ? top[0] : top[1];
+  for (int m = 32; m > 0; m >>= 1) {
+    const uint32_t other = __shfl_xor(bits, m);
+    bits = bits > other ? bits : other;
+  }
+  bits = uni(bits);
+  const bool finite = bits < kInf;            // of every value: the usual case
+  float amax = widen<TYPE>(bits);
+  if (!finite) {                              // the largest of those that are
+    amax = 0.f;
+    for (int c = 0; c < chunks; ++c) {
+      if (chunks > 1) load(c * kChunk);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = fabsf(widen<TYPE>(x[i][e] & 0xffffu)), hi = fabsf(widen<TYPE>(x[i][e] >> 16));
+          if (finite_bits(lo)) amax = fmaxf(amax, lo);
+          if (finite_bits(hi)) amax = fmaxf(amax, hi);
+        }
+    }
+    for (int m = 32; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+  }
 
   const bool kept = r0 > 0 && 448.f * s_old >= amax;
   const float scale = kept ? s_old : needed_scale(amax);
   const Divider by(scale);
+  const bool plain = uni(finite && by.pow2);
   if (r0 > 0 && !kept) {
-    for (int r = sub; r < r0; r += kRows) {
-      const uint64_t at = page + (uint64_t)(r * a.layer.token_stride);
-      u32x2 c = gload<u32x2>(at);
+    for (int q0 = 0; q0 < r0; q0 += kRows * kOld) {        // kOld loads in flight; more would cost registers, and waves, in every call
+      u32x2 old[kOld];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[e], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[e], true);
-        c[e] = pack4(by(lo[0] * s_old), by(lo[1] * s_old), by(hi[0] * s_old), by(hi[1] * s_old));
+      for (int i = 0; i < kOld; ++i) {
+        const int r = q0 + i * kRows + sub;
+        old[i] = u32x2{0, 0};
+        if (r < r0) old[i] = gload<u32x2>(page + (uint64_t)(r * a.layer.token_stride));
       }
-      gstore<u32x2>(at, c);
+#pragma unroll
+      for (int i = 0; i < kOld; ++i) {
+        const int r = q0 + i * kRows + sub;
+        if (r < r0) {
+          u32x2 c = old[i];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[e], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[e], true);
+            c[e] = pack4(by(lo[0] * s_old), by(lo[1] * s_old), by(hi[0] * s_old), by(hi[1] * s_old));
+          }
+          gstore<u32x2>(page + (uint64_t)(r * a.layer.token_stride), c);
+        }
+      }
     }
   }
   for (int c = 0; c < chunks; ++c) {
     if (chunks > 1) load(c * kChunk);
+    if (plain) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int r = c * kChunk + i * kRows + sub;
+        if (r < n) gstore<u32x2>(page + (uint64_t)((r0 + r) * a.layer.token_stride), u32x2{pack4_scaled<TYPE>(x[i][0], x[i][1], scale), pack4_scaled<TYPE>(x[i][2], x[i][3], scale)});
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int r = c * kChunk + i * kRows + sub;
