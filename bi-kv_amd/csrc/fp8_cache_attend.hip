@@ -1033,10 +1033,12 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
     take_z(0);
+    if constexpr (TYPE == 1) {
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-      if (j >= D / 32) __builtin_amdgcn_sched_group_barrier(0x2, 512 / D, 0);
+      for (int j = 0; j < D / 16; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (j >= D / 32) __builtin_amdgcn_sched_group_barrier(0x2, 512 / D, 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     read_ks(1);
@@ -1124,11 +1126,15 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         read_v(1, s2, dt);
       }
     weights(1);
+    // with fp16's twice as many products the order is given: a 4096-token prompt takes 276 us, 297 in the compiler's own
+    // order; bf16's is as fast in the compiler's
+    if constexpr (TYPE == 1) {
 #pragma unroll
-    for (int i = 0; i < 2 * (D / 32); ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, TYPE == 1 ? 2 : 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x2, 768 / D, 0);
+      for (int i = 0; i < 2 * (D / 32); ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 768 / D, 0);
+      }
     }
     if (edge) blank(1);
     pack(1);
@@ -1268,7 +1274,6 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
   if (mean <= 64 && (all / m + n_seqs) * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
     p.form = mean <= 16 ? ATTEND_FEW_16 : mean <= 32 ? ATTEND_FEW_32 : ATTEND_FEW_64;
     p.rows = m;
-    p.tiles = all / m + n_seqs;
     p.tiles = all / m + n_seqs;
     const int waves = m == 64 ? 4 : 8;
     p.heads_per_group = heads < waves ? heads : waves;
