@@ -105,6 +105,8 @@ class FP8KVCache:
             if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
                 raise RuntimeError(f"{name} must be [rows, {heads if heads is not None else 'heads'}, {self.head_dim}], got {list(shape)}")
             raise RuntimeError(f"{name}: the values of a head must be contiguous")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient, and the cache's calls record none: detach it or call under torch.no_grad()")
         return stride
 
     def _batch(self, rows, page_table, kv_lens, q_starts):

@@ -84,8 +84,8 @@ static int check_batch(const bikv_fp8_cache* c, int32_t layer, const bikv_seq_ba
     return fail(BIKV_EINVAL, "without q_starts every sequence has one row: n_rows %lld, n_seqs %lld", (long long)b->n_rows, (long long)b->n_seqs);
   if (b->page_table_stride < b->max_pages) return fail(BIKV_EINVAL, "page_table_stride %lld is less than max_pages %lld", (long long)b->page_table_stride, (long long)b->max_pages);
   if (b->n_seqs >= (int64_t(1) << 24) || b->n_rows >= (int64_t(1) << 30)) return fail(BIKV_ERANGE, "more than 2^24 sequences or 2^30 rows");
-  if (b->max_pages >= (int64_t(1) << 31) / c->page_tokens)
-    return fail(BIKV_ERANGE, "max_pages * page_tokens must stay below 2^31 (got %lld * %d)", (long long)b->max_pages, c->page_tokens);
+  if (b->max_pages > (int64_t(1) << 30) / c->page_tokens)
+    return fail(BIKV_ERANGE, "max_pages * page_tokens must not be more than 2^30 (got %lld * %d)", (long long)b->max_pages, c->page_tokens);
   seq->table = b->page_table;
   seq->table_stride = b->page_table_stride;
   seq->kv_lens = b->kv_lens;
@@ -147,7 +147,7 @@ static int plan_call(const bikv_fp8_cache* c, const bikv_seq_batch* b, int32_t q
   if (q_heads <= 0 || q_heads % c->heads != 0) return fail(BIKV_EINVAL, "q_heads %d must be a positive multiple of kv_heads %d", q_heads, c->heads);
   if (b->n_seqs < 0 || b->n_rows < 0 || b->max_pages < 0) return fail(BIKV_EINVAL, "negative n_seqs, n_rows or max_pages");
   if (b->n_seqs >= (int64_t(1) << 24) || b->n_rows >= (int64_t(1) << 30) || b->n_rows * (q_heads / c->heads) >= (int64_t(1) << 31) ||
-      b->max_pages >= (int64_t(1) << 31) / c->page_tokens)
+      b->max_pages > (int64_t(1) << 30) / c->page_tokens)
     return fail(BIKV_ERANGE, "too many sequences, rows or pages for one call");
   *plan = AttendPlan();
   if (b->n_seqs == 0 || b->n_rows == 0) return BIKV_OK;

@@ -268,8 +268,11 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), (NT <= 2 ? 2 :
     const int rows = uni((int)((int64_t)seq.n * G - (int64_t)tile * kM < kM ? (int64_t)seq.n * G - (int64_t)tile * kM : kM));
     const int len = uni(seq.len);
     const int before = a.causal ? uni(seq.len - seq.n) : 0;     // keys older than the call's own (negative: some rows see none)
-    if (step0 == 0 && !whole)
-      join = {seq.first, tile, rows, (int)((at + steps - 1) / line.per) - slot + 1, 2 * slot + (first_of_share ? 0 : 1)};
+    if (step0 == 0 && !whole) {
+      int parts = (int)((at + steps - 1) / line.per) - slot + 1;
+      if (parts > a.slots - slot) parts = a.slots - slot;          // row numbers that make no sense may have wrapped the line's length
+      join = {seq.first, tile, rows, parts, 2 * slot + (first_of_share ? 0 : 1)};
+    }
 
     const int last_tok = uni((int)divide((uint32_t)(tile * kM + rows - 1), a.group));
     const int first_tok = uni((int)divide((uint32_t)(tile * kM), a.group));

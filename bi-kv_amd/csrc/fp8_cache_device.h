@@ -25,10 +25,6 @@ template <class T>
 __device__ __forceinline__ void gstore(uint64_t addr, T v) {
   *(BIKV_G T*)addr = v;
 }
-template <class T>
-__device__ __forceinline__ void gstore_nt(uint64_t addr, T v) {
-  __builtin_nontemporal_store(v, (BIKV_G T*)addr);
-}
 
 __device__ __forceinline__ void raise_flag(uint32_t* status, int slot) {
   *(volatile BIKV_G uint32_t*)(status + slot) = 1u;
@@ -64,10 +60,9 @@ __device__ __forceinline__ Seq read_seq(const SeqArgs& s, int64_t b) {
   return r;
 }
 
-// The largest b < n_seqs whose first slot f(b) = floor(q_starts[b] * mul / div) + per * b is not beyond
-// `slot`. f grows with b, so a 64-way search by a whole wave finds it in one step for 64 sequences, two
-// for 4096. With row numbers that do not grow the result is some b in range: callers check that the slot
-// is one of that sequence's.
+// The largest b < n_seqs whose first_slot(b) is not beyond `slot`. first_slot grows with b, so a 64-way search by a
+// whole wave finds it in one step for 64 sequences, two for 4096. With row numbers that do not grow
+// the result is some b in range: callers check that the slot is one of that sequence's.
 template <class F>
 __device__ __forceinline__ int64_t find_seq(int64_t n_seqs, int64_t slot, int lane, F first_slot) {
   int64_t lo = 0, n = n_seqs;       // the answer is in [lo, lo + n)

@@ -18,7 +18,7 @@ struct SeqArgs {
   const int64_t* q_starts;   // n_seqs + 1 row numbers, or null: sequence b owns row b
   int64_t n_seqs;
   int64_t n_rows;            // rows of the caller's tensors
-  int64_t max_len;           // max_pages * page_tokens, below 2^31
+  int64_t max_len;           // max_pages * page_tokens, at most 2^30: a few steps more still fit an int
 };
 
 // One layer of the cache.

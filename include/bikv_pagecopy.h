@@ -481,6 +481,7 @@ int bikv_nhd_store_token_major(const bikv_nhd* pool, void* tm, int64_t tm_bytes,
  * tensors, for append more rows than tokens) is skipped as a whole and raises BIKV_ST_SRC_RANGE; a page id outside the pool
  * raises BIKV_ST_PAGE_ID and its tokens are left out. Asynchronous on `stream`, no allocation, graph-capturable.
  * Row and head strides are in elements, multiples of 8; addresses are 16-byte aligned; a head's values are contiguous.
+ * max_pages * page_tokens is at most 2^30, n_rows below 2^30, n_seqs below 2^24 (BIKV_ERANGE).
  * ------------------------------------------------------------------------------------------ */
 typedef struct bikv_fp8_cache bikv_fp8_cache; /* opaque; host memory only */
 
