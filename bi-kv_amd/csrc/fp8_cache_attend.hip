@@ -48,7 +48,14 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {      // nearest, ties to even
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
-__device__ __forceinline__ float half_of(uint32_t pair, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> (16 * i))); }
+// x less the fp16 value in the pair's low (0) or high (1) half: one instruction, where widening and subtracting are two.
+template <int HIGH>
+__device__ __forceinline__ float less_half(float x, uint32_t pair) {
+  float y;
+  if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(pair), "v"(x));
+  else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(pair), "v"(x));
+  return y;
+}
 template <int TYPE>
 __device__ __forceinline__ uint32_t narrow(float a, float b) {
   if constexpr (TYPE == 0)
@@ -482,7 +489,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), (NT <= 2 ? 2 :
             const float f0 = s[t][i][2 * c], f1 = s[t][i][2 * c + 1];
             const uint32_t y = pack_f16(f0, f1);
             p[t][i / 2][2 * (i & 1) + c] = y;
-            if constexpr (TYPE == 1) p_low[t][i / 2][2 * (i & 1) + c] = pack_f16(f0 - half_of(y, 0), f1 - half_of(y, 1));
+            if constexpr (TYPE == 1) p_low[t][i / 2][2 * (i & 1) + c] = pack_f16(less_half<0>(f0, y), less_half<1>(f1, y));
           }
       }
       if (more) wait_vmem<4 + kCopies>();                        // all but what has just been asked for
@@ -1109,7 +1116,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int i = 0; i < 16; i += 2) {
         const uint32_t y = pack_f16(s[kb][i], s[kb][i + 1]);
         pf[kb][i / 8][(i & 7) / 2] = y;
-        if constexpr (TYPE == 1) pf_low[kb][i / 8][(i & 7) / 2] = pack_f16(s[kb][i] - half_of(y, 0), s[kb][i + 1] - half_of(y, 1));
+        if constexpr (TYPE == 1) pf_low[kb][i / 8][(i & 7) / 2] = pack_f16(less_half<0>(s[kb][i], y), less_half<1>(s[kb][i + 1], y));
       }
     };
     auto gather = [&](int kb, int s2, int dt) {
