@@ -943,7 +943,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 #pragma unroll
     for (int c = 0; c < 8; ++c) raw_v[c] = gload<uint32_t>(vbase + m.off[v_key(c)] + v_at);
   };
-  auto put = [&](int t, int buf, const Meta& m) {
+  auto put = [&](int t, int buf, const Meta& m, bool gone) {
     static_assert(256 / kPieces % 16 == 0, "the rows of a thread's pieces share their swizzle");
     const uint32_t k_at = opaque(k_write);
 #pragma unroll
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         const u32x2 lo = widen4<TYPE>(raw_k[i][2 * e]), hi = widen4<TYPE>(raw_k[i][2 * e + 1]);
         at_k(buf, (k_at ^ (16 * e)) + i * (256 / kPieces) * kKRow) = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
-    if ((t + 1) * kKeys > all || m.gone) {
+    if ((t + 1) * kKeys > all || gone) {
       // bytes of keys that nobody sees become zero, and so does a NaN: the rows that see its key get it at the end
       uint32_t any = 0;
 #pragma unroll
@@ -997,8 +997,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int c = 0; c < 16; ++c) o[i][c] *= by;
   };
 
-  auto compute = [&](int t, int buf, const Meta& meta) {
-    const int r = uni(meta.r);
+  auto compute = [&](int t, int buf, const Meta& meta, int r, bool gone) {
     if (r != r_exp) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -1006,7 +1005,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         for (int c = 0; c < 16; ++c) o[i][c] = ldexpf(o[i][c], r_exp - r);
       r_exp = r;
     }
-    const bool edge = (t + 1) * kKeys > wave_all || uni(meta.gone);
+    const bool edge = (t + 1) * kKeys > wave_all || gone;
     // Operands are read from LDS half a step ahead of the products that use them, each into the registers of the
     // operand just used; left alone, the compiler reads each one right before its product and waits for it.
     f32x16 s[2];
@@ -1038,6 +1037,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int i = 0; i < 16; ++i) s[kb][i] = fmaf(s[kb][i], ks[kb][i / 4][i & 3], -from);
     };
     read_ks(0);
+    if constexpr (D == 64) read_ks(1);             // the larger head has no registers for both
     __builtin_amdgcn_sched_barrier(0);
     // the first half's z stand between the second half's products
 #pragma unroll
@@ -1051,7 +1051,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    read_ks(1);
+    if constexpr (D != 64) read_ks(1);
     __builtin_amdgcn_sched_barrier(0);
     take_z(1);
     uint32_t hidden = 0;
@@ -1168,7 +1168,8 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     find_exponent(metas[wave]);
     lds_barrier();
     finish(0, metas[wave]);
-    put(t0, 0, metas[0]);
+    int gone = uni(metas[0].gone);
+    put(t0, 0, metas[0], gone);
     lds_barrier();
     for (int t = t0; t < t1; ++t) {
       const int i = t - t0, ahead = (i & 4) ^ 4;   // ahead: where the ring has the next four steps
@@ -1182,9 +1183,12 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       } else if ((i & 3) == 3) {
         finish(ahead, metas[ahead + wave]);
       }
+      const int r_read = metas[i & 7].r, gone_read = metas[(i + 1) & 7].gone;      // read here: their wait is the one that bring has anyway
       bring(metas[(i + 1) & 7]);
-      if (t * kKeys < wave_seen) compute(t, i & 1, metas[i & 7]);
-      if (t + 1 < t1) put(t + 1, (i & 1) ^ 1, metas[(i + 1) & 7]);
+      const int r = uni(r_read), gone_next = uni(gone_read);
+      if (t * kKeys < wave_seen) compute(t, i & 1, metas[i & 7], r, gone);
+      if (t + 1 < t1) put(t + 1, (i & 1) ^ 1, metas[(i + 1) & 7], gone_next);
+      gone = gone_next;
       lds_barrier();
     }
     wait_vmem<0>();                                // no copy into LDS outlives the workgroup
