@@ -88,7 +88,7 @@ __device__ __forceinline__ int scale_exponent(float s) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---------------------------------------------------------------------------------------------
-// Few rows per sequence: a workgroup takes a tile of 16, 32 or 64 rows over a run of key steps, its waves the KV
+// Few rows per sequence: a workgroup takes a tile of 16 or 32 rows over a run of key steps, its waves the KV
 // heads; where there are more waves than heads, several waves share a head and take its steps in turn.
 //
 // Bound by memory: every byte of K and V is read once per row tile. Each wave copies its own steps' rows into its own part
@@ -108,7 +108,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 template <int D, int TYPE, int NT, int NK>
 struct Few {
   static constexpr int kM = 16 * NT;       // rows of a tile
-  static constexpr int kWaves = NT <= 2 ? 8 : 4;   // 8 waves of 256 registers fill a CU, 4 of 512
+  static constexpr int kWaves = 8;         // of 256 registers: they fill a CU
   static constexpr int kKeys = 16 * NK;    // keys of a step
   static constexpr int kDT = D / 16;       // bytes of a V row per lane, and row tiles of O^T
   static constexpr int kChunks = D / 16;   // 16-byte pieces of a key's row
@@ -194,7 +194,7 @@ __device__ __forceinline__ int64_t seq_at(const AttendArgs& a, uint32_t x, int l
 }
 
 template <int D, int TYPE, int NT, int NK>
-__global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), (NT <= 2 ? 2 : 1)) void fp8_attend_few_kernel(const AttendArgs a) {
+__global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_attend_few_kernel(const AttendArgs a) {
   using C = Few<D, TYPE, NT, NK>;
   constexpr int kM = C::kM, kKeys = C::kKeys, kDT = C::kDT, kChunks = C::kChunks, kCopies = C::kCopies, kWaves = C::kWaves;
   constexpr int kQK = D / 32;              // matrix steps of q . k
@@ -1284,15 +1284,20 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
   AttendPlan p = {};
   const int64_t all = n_rows * group;                      // rows of one KV head
   const int64_t mean = (all + n_seqs - 1) / n_seqs;
-  const int m = mean <= 16 ? 16 : mean <= 32 ? 32 : 64, keys = m == 16 ? 64 : 32;
-  if (mean <= 64 && (all / m + n_seqs) * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
-    p.form = mean <= 16 ? ATTEND_FEW_16 : mean <= 32 ? ATTEND_FEW_32 : ATTEND_FEW_64;
+  // Few rows: the fewer, the more of a wide tile would be computed for nothing. Rows of a sequence on average, 64 sequences of
+  // 3500 tokens, 8 KV heads: 16 rows 113 us against 137 as many rows; 28 rows (4 heads) 75 against 116; 32 rows 144
+  // against 141; a 64-row tile of this kind was 2 to 3 times slower than the many rows' and is not there.
+  const int m = mean <= 16 ? 16 : 32, keys = m == 16 ? 64 : 32;
+  if (mean <= 32 && (all / m + n_seqs) * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
+    p.form = m == 16 ? ATTEND_FEW_16 : ATTEND_FEW_32;
     p.rows = m;
     p.tiles = all / m + n_seqs;
-    const int waves = m == 64 ? 4 : 8;
+    const int waves = 8;
     p.heads_per_group = heads < waves ? heads : waves;
-    if (max_len <= 2048) {
-      // a workgroup per tile; with few of them a head gets more waves
+    if (max_len <= 1024) {
+      // A workgroup per tile, no second launch: 11.5 us against 16 for a sequence of 500 tokens, 15 against 16 at 1000; at 1500
+      // shares are ahead (18.7 against 17.1), and at 4000 by half (35 against 22). Where there are few tiles a head gets
+      // more waves, of more workgroups: 8 sequences of up to 2000 tokens take 22 us, 103 without.
       while (p.heads_per_group > 1 && p.tiles * ((heads + p.heads_per_group - 1) / p.heads_per_group) < 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
       p.slots = 0;
     } else {
@@ -1306,7 +1311,9 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
     p.tiles = all / kManyRows + n_seqs;
-    int64_t parts = (512 + p.tiles * heads / 2) / (p.tiles * heads);       // two workgroups to a CU
+    // Two workgroups to a CU: 300 new tokens of each of 2 sequences of 3500, 4 KV heads, take 52 us in 6 parts, 119 in one and 66
+    // in 12; parts of four steps at least.
+    int64_t parts = (512 + p.tiles * heads / 2) / (p.tiles * heads);
     const int64_t steps = (max_len + kManyKeys - 1) / kManyKeys;
     if (parts > steps / 4) parts = steps / 4;
     p.slots = (int32_t)(parts < 1 ? 1 : parts);
@@ -1328,7 +1335,6 @@ static hipError_t launch_form(const AttendPlan& p, const AttendArgs& a, hipStrea
   switch (p.form) {
     case ATTEND_FEW_16: return launch_few<D, TYPE, 1, 4>(p, a, s);
     case ATTEND_FEW_32: return launch_few<D, TYPE, 2, 2>(p, a, s);
-    case ATTEND_FEW_64: return launch_few<D, TYPE, 4, 2>(p, a, s);
     default: break;
   }
   hipLaunchKernelGGL((fp8_attend_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * p.slots)), dim3(256), 0, s, a);

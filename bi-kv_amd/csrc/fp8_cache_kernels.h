@@ -75,7 +75,7 @@ struct AttendArgs {
   int64_t tiles;             // row tiles of the launch
   uint32_t* status;
 };
-enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_FEW_64 = 2, ATTEND_MANY = 3 };
+enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_MANY = 2 };
 struct AttendPlan {
   int form;
   int rows;                  // rows of a tile
