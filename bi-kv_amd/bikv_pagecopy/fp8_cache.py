@@ -185,7 +185,7 @@ class FP8KVCache:
                 raise RuntimeError("out must not share memory with q")
         heads = shape[1]
         lse = q.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
-        key = (shape[0], heads, page_table.shape)
+        key = (shape[0], heads, page_table.shape, q_starts is None)
         need = self._workspace.get(key)
         if need is None:                     # a size that follows from these numbers alone
             need = _lib.check(self._lib.bikv_fp8_attend_workspace(self._h, batch, heads))

@@ -151,7 +151,7 @@ static int plan_call(const bikv_fp8_cache* c, const bikv_seq_batch* b, int32_t q
     return fail(BIKV_ERANGE, "too many sequences, rows or pages for one call");
   *plan = AttendPlan();
   if (b->n_seqs == 0 || b->n_rows == 0) return BIKV_OK;
-  *plan = plan_fp8_attend(c->head_dim, c->heads, q_heads / c->heads, b->n_seqs, b->n_rows, b->max_pages * c->page_tokens);
+  *plan = plan_fp8_attend(c->heads, q_heads / c->heads, !b->q_starts, b->n_seqs, b->n_rows, b->max_pages * c->page_tokens);
   if (plan->tiles * c->heads * (plan->form == ATTEND_MANY ? plan->slots * 32 : 1) >= (int64_t(1) << 31))
     return fail(BIKV_ERANGE, "too many rows times heads for one call");
   return BIKV_OK;

@@ -149,16 +149,17 @@ __device__ __forceinline__ uint32_t weight_of(const AttendArgs& a, int64_t b) {
   return tiles_of(s, a.group, M) * steps_of(s, KEYS);
 }
 
-// The number of the row tile that sequence b's first row begins, if every sequence may leave one tile unfilled: a rising
-// function of b with room for all of its tiles.
+// The number of the row tile that sequence b's first row begins: with one token each the sequences have as many tiles
+// each; else, if every sequence may leave one tile unfilled, a rising function of b with room for all of its tiles.
 template <int M>
 __device__ __forceinline__ int64_t first_tile(const AttendArgs& a, int64_t b) {
-  int64_t q = b;
-  if (a.seq.q_starts) {
-    q = a.seq.q_starts[b];
-    q = q < 0 ? 0 : q > a.seq.n_rows ? a.seq.n_rows : q;
-  }
+  if (!a.seq.q_starts) return b * ((a.group.d + M - 1) / M);
+  int64_t q = a.seq.q_starts[b];
+  q = q < 0 ? 0 : q > a.seq.n_rows ? a.seq.n_rows : q;
   return q * a.group.d / M + b;
+}
+static int64_t tiles_in_all(bool one_each, int group, int64_t n_seqs, int64_t n_rows, int m) {
+  return one_each ? n_seqs * ((group + m - 1) / m) : n_rows * group / m + n_seqs;
 }
 
 // The line's length (the host sees to it that it stays below 2^31).
@@ -1280,7 +1281,7 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
 }
 
 // ---------------------------------------------------------------------------------------------
-AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, int64_t n_rows, int64_t max_len) {
+AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, int64_t n_rows, int64_t max_len) {
   AttendPlan p = {};
   const int64_t all = n_rows * group;                      // rows of one KV head
   const int64_t mean = (all + n_seqs - 1) / n_seqs;
@@ -1288,17 +1289,20 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
   // 3500 tokens, 8 KV heads: 16 rows 113 us against 137 as many rows; 28 rows (4 heads) 75 against 116; 32 rows 144
   // against 141; a 64-row tile of this kind was 2 to 3 times slower than the many rows' and is not there.
   const int m = mean <= 16 ? 16 : 32, keys = m == 16 ? 64 : 32;
-  if (mean <= 32 && (all / m + n_seqs) * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
+  const int64_t tiles = tiles_in_all(one_each, group, n_seqs, n_rows, m);
+  if (mean <= 32 && tiles * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
     p.form = m == 16 ? ATTEND_FEW_16 : ATTEND_FEW_32;
     p.rows = m;
-    p.tiles = all / m + n_seqs;
+    p.tiles = tiles;
     const int waves = 8;
     p.heads_per_group = heads < waves ? heads : waves;
     if (max_len <= 1024) {
       // A workgroup per tile, no second launch: 11.5 us against 16 for a sequence of 500 tokens, 15 against 16 at 1000; at 1500
-      // shares are ahead (18.7 against 17.1), and at 4000 by half (35 against 22). Where there are few tiles a head gets
-      // more waves, of more workgroups: 8 sequences of up to 2000 tokens take 22 us, 103 without.
-      while (p.heads_per_group > 1 && p.tiles * ((heads + p.heads_per_group - 1) / p.heads_per_group) < 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
+      // shares are ahead (18.7 against 17.1), and at 4000 by half (35 against 22). Where there are few tiles a head
+      // gets more waves, of more workgroups: 8 sequences of up to 2000 tokens take 22 us, 103 without; but
+      // no more workgroups than CUs, each of which holds one (42 short sequences 12.6 us, 19.4 in twice as many).
+      auto groups = [&](int32_t per) { return tiles * ((heads + per - 1) / per); };
+      while (p.heads_per_group > 1 && groups((p.heads_per_group + 1) / 2) <= 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
       p.slots = 0;
     } else {
       // one workgroup for each of the 256 CUs, which is what one holds of this size
@@ -1310,7 +1314,7 @@ AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, i
   } else {
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
-    p.tiles = all / kManyRows + n_seqs;
+    p.tiles = tiles_in_all(one_each, group, n_seqs, n_rows, kManyRows);
     // Two workgroups to a CU: 300 new tokens of each of 2 sequences of 3500, 4 KV heads, take 52 us in 6 parts, 119 in one and 66
     // in 12; parts of four steps at least.
     int64_t parts = (512 + p.tiles * heads / 2) / (p.tiles * heads);

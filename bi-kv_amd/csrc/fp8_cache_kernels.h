@@ -85,8 +85,8 @@ struct AttendPlan {
   int64_t tiles;
   int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
 };
-// The form a call takes, from what the host knows of it alone.
-AttendPlan plan_fp8_attend(int head_dim, int heads, int group, int64_t n_seqs, int64_t n_rows, int64_t max_len);
+// The form a call takes, from what the host knows of it alone. one_each: no row numbers, a sequence has one row.
+AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, int64_t n_rows, int64_t max_len);
 hipError_t launch_fp8_attend(const AttendPlan& plan, int head_dim, int type, const AttendArgs& a, hipStream_t stream);
 
 }  // namespace bikv
