@@ -12,7 +12,9 @@
 // takes its P^T operand in, as long as V^T's keys are put in the same order: P never crosses lanes or
 // memory. K is widened to q's type and Q K^T is exact up to fp32 sums. P is rounded to fp16 (11 bits; bf16's 8 would
 // cost as much as the output's own rounding): p vs 2^(8 - r) with r the largest exponent of vs so far, so that
-// neither a page's scale nor a small p leaves fp16's range; the exponent comes off again at the end.
+// neither a page's scale nor a small p leaves fp16's range; the exponent comes off again at the end. Where q is fp16, 11 bits
+// would cost as much as the output's own rounding, and P goes as the sum of two fp16 numbers. A page whose V scale is
+// below 2^-22 of the largest among the keys read before it loses bits against that page's values, not against the larger ones.
 // l sums the unrounded p.
 #include "fp8_cache_device.h"
 
@@ -90,6 +92,11 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // ---------------------------------------------------------------------------------------------
 // Few rows per sequence: a workgroup takes a tile of 16 or 32 rows over a run of key steps, its waves the KV
 // heads; where there are more waves than heads, several waves share a head and take its steps in turn.
+//
+// Measured, with fp8_join_few_kernel: 64 sequences of 1024 to 8192 tokens, 64 query and 8 KV heads of 128, bf16, one new token
+// each: 612 MB in 121 + 7 us, 5.05 TB/s while the first kernel runs; 3 of 32k, 32 heads: 186 MB in 37 + 8 us; 24 of up to 5000
+// with up to 5 new tokens, 28 and 4 heads: 69 MB in 34 + 6 us; one of 777, 12 and 2 heads: 13.5 us, where what counts is the
+// chain of lookups (lengths, page ids, scales and rows) and how long code and data take to arrive.
 //
 // Bound by memory: every byte of K and V is read once per row tile. Each wave copies its own steps' rows into its own part
 // of LDS (global_load_lds, 16 bytes a lane, whole rows) and never waits for another wave while it goes: scales and the next
@@ -771,9 +778,20 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // Many rows per sequence: a workgroup of four waves does 128 rows of one KV head, 32 a wave, over the
 // keys 64 at a time.
 //
-// Bound by the matrix cores (4 D flops per visible row and key) and by what stands beside them: one exp2 per row
-// and key, and the widening of K and V, which is done once per workgroup: two waves bring K, two V, as
-// bytes into registers while the step before is computed, then widened into LDS: K as [key][D] in
+// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 247 us (556 TFLOP/s); 6 chunks of
+// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 760 us (731 TFLOP/s); 5 of up to 700 tokens and
+// 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 38 + 8 us.
+//
+// Bound by what the matrix products (4 D flops per visible row and key), the softmax beside them (an exp2 and some six other
+// instructions per row and key) and the reads from LDS (a wave's 32 rows need the whole step's K and V) take together: of the
+// second case's time the matrix cores are busy 29 %, the vector units 44 %, LDS 38 %, and two waves to a SIMD, all that
+// registers allow, overlap little of it. So products and softmax are interleaved by halves of a step, and what a step needs from
+// LDS is read half a step ahead. For 64-wide heads it is the length of that chain, 2.3 us a step, also for a wave that has
+// its SIMD to itself. fp16 rows carry P in two halves (see the file's head: P has 11 bits, as much as the output), which makes
+// twice the products of O.
+//
+// K and V are widened once per workgroup. Threads bring them as bytes into registers while the step before is computed, K as
+// 16-byte pieces of rows, V as four bytes of each of eight keys, and put them into LDS afterwards: K as [key][D] in
 // q's type, V transposed as [D][key] in fp16 with the keys in the order in which P lies in the lanes. 16-byte
 // pieces of a row are XOR-ed with the row number, so that neither the writes nor the reads of a column meet in
 // a bank. Two LDS buffers, one barrier a step.
@@ -783,7 +801,7 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
-constexpr float kSlack = 4.f;           // p 2^kPShift vs 2^-r < 2^(4 + 8 + 1), in fp16's range
+constexpr float kSlack = 4.f;           // p 2^kPShift vs 2^-r < 2^(4 + 8 + 1), in fp16's range; with 0, chunks of 900 behind 8192 tokens take 704 us, with 4 682
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -1315,12 +1333,24 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
     p.tiles = tiles_in_all(one_each, group, n_seqs, n_rows, kManyRows);
-    // Two workgroups to a CU: 300 new tokens of each of 2 sequences of 3500, 4 KV heads, take 52 us in 6 parts, 119 in one and 66
-    // in 12; parts of four steps at least.
-    int64_t parts = (512 + p.tiles * heads / 2) / (p.tiles * heads);
+    // Parts of a tile's keys. The chip holds 512 of these workgroups, two to a CU, so `n` of them take ceil(n / 512) rounds of their
+    // steps, and some two steps more to begin and to end (two again where empty workgroups, of tiles that sequences may have
+    // and these do not, take a place first); the parts' sums are written and read again, 115 of them in a step's time. 33 sequences of 40 to 64 rows over 4000 keys, 8 KV heads: 243 us in one part, 184 in three; 300 new
+    // tokens of each of 2 sequences of 3500, 4 KV heads: 52 us in 6 parts, 119 in one and 66 in 12. From 1024 tiles on the rounds
+    // even out by themselves. Parts have four steps at least.
+    const int64_t tiles_likely = one_each ? p.tiles : all / kManyRows + n_seqs / 2, n = heads * (tiles_likely > n_seqs ? tiles_likely : n_seqs);
     const int64_t steps = (max_len + kManyKeys - 1) / kManyKeys;
-    if (parts > steps / 4) parts = steps / 4;
-    p.slots = (int32_t)(parts < 1 ? 1 : parts);
+    p.slots = 1;
+    if (n < 1024) {
+      int64_t least = -1;
+      for (int64_t parts = 1; parts <= 64 && (parts == 1 || parts <= steps / 4); ++parts) {
+        const int64_t cost = (n * parts + 511) / 512 * ((steps + parts - 1) / parts + 2) + (parts > 1 ? n * parts / 115 + 2 : 0) + (p.tiles * heads * parts > 512 ? 2 : 0);
+        if (least < 0 || cost < least) {
+          least = cost;
+          p.slots = (int32_t)parts;
+        }
+      }
+    }
     p.part_rows = p.slots > 1 ? p.tiles * heads * p.slots * kManyRows : 0;
   }
   return p;

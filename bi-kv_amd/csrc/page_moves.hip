@@ -1,7 +1,9 @@
 // Page copies inside a layered pool (gfx950): page dst_ids[i] becomes a copy of page src_ids[i], every plane of it,
 // payload and scale tiles, in one launch.
 //
-// Bound by memory: each byte is read once and written once. The shape is the one the pool's movers run
+// Bound by memory: each byte is read once and written once. Measured: 450 pages of 80 layers of 8-bit KV with scales, 2.36 GB read
+// and written, in 460 us (5.1 TB/s; a large torch copy in the same memory 4.7); 2 pages of 28 layers in 2.7 us. Loads and stores
+// with and without the non-temporal and system-scope hints run alike. The shape is the one the pool's movers run
 // fastest with: every 64 vectors of a tile are a workgroup of one wave, one vector per lane, the entry's ids and the
 // plane's base by scalar loads. A page's planes follow each other in the grid, so that neighbouring
 // workgroups touch planes gigabytes apart. A gather into staging and a scatter out of it would move the same bytes
