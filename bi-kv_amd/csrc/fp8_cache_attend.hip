@@ -778,9 +778,9 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // Many rows per sequence: a workgroup of four waves does 128 rows of one KV head, 32 a wave, over the
 // keys 64 at a time.
 //
-// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 247 us (556 TFLOP/s); 6 chunks of
-// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 760 us (731 TFLOP/s); 5 of up to 700 tokens and
-// 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 38 + 8 us.
+// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 242 us (568 TFLOP/s); 6 chunks of
+// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 750 us (741 TFLOP/s); 5 of up to 700 tokens and
+// 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 39 us.
 //
 // Bound by what the matrix products (4 D flops per visible row and key), the softmax beside them (an exp2 and some six other
 // instructions per row and key) and the reads from LDS (a wave's 32 rows need the whole step's K and V) take together: of the
