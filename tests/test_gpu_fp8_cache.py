@@ -355,6 +355,65 @@ def test_attend(bk, cuda, case, P, H, D, dtype):
     _run(w, w.randn(w.Hq, 1.5), causal=False)
 
 
+SHAPES = [
+    # lens, new tokens (None: one each, without row numbers), KV heads, q heads per KV head, head size
+    ([70, 300, 5], None, 2, 40, 128),                                # one token, more rows than a narrow tile has
+    ([500, 130], None, 1, 200, 64),                                  # and more than a wide one has
+    ([600, 64, 33, 9], [5, 8, 6, 7], 2, 8, 128),                     # 40 to 64 rows
+    ([100 + 4 * i for i in range(33)], [5 + i % 4 for i in range(33)], 4, 8, 64),
+    ([5 + 3 * i for i in range(60)], None, 9, 2, 64),                # heads that do not fill their workgroups
+    ([200, 77], None, 12, 1, 128),
+    ([200, 77], [2, 3], 17, 5, 64),
+    ([40] * 53, [1 + i % 2 for i in range(53)], 4, 8, 128),          # as many workgroups as CUs, and more
+    ([30 + i for i in range(130)], None, 3, 6, 64),
+    ([1024, 1000], None, 2, 4, 128), ([1025, 17], None, 2, 4, 128),  # either side of the length from which work is cut
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("wide", [0, 9000])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_attend_whichever_way_the_work_is_cut(bk, cuda, case, wide, dtype):
+    lens, news, H, G, D = SHAPES[case]
+    w = World(bk, cuda, lens, news or [1] * len(lens), P=16, H=H, D=D, Hq=G * H, dtype=dtype, seed=50 + case, ragged=news is not None, wide=wide)
+    _run(w, w.randn(w.Hq, 1.5), causal=True)
+    _run(w, w.randn(w.Hq, 1.5), causal=False)
+
+
+def test_row_numbers_that_fall_and_overlap_do_no_harm(bk, cuda):
+    """Sequences whose rows make no sense are skipped and reported; those whose rows are others', too, may hold either's result."""
+    for lens, starts in (([300, 40, 300], [0, 20, 5, 25]), ([70, 70, 70, 70], [0, 9, 0, 9, 0]), ([3000, 3000, 10], [0, 25, 0, 25])):
+        for wide in (0, 9000):
+            w = World(bk, cuda, lens, [1] * len(lens), H=2, Hq=8, seed=70, wide=wide)
+            w.rows = max(starts)
+            q = w.randn(8).to(cuda)
+            k = w.randn(2).to(cuda)
+            s = torch.tensor(starts, device=cuda)
+            w.cache.attend(1, q, w.table_d, w.lens_d, s)
+            with pytest.raises(RuntimeError):
+                w.cache.check()
+            w.cache.append(1, k, k, w.table_d, w.lens_d, s)
+            with pytest.raises(RuntimeError):
+                w.cache.check()
+    w = World(bk, cuda, [100, 20], [3, 1], H=2, Hq=8, seed=71)
+    q = w.randn(8)
+    _run(w, q)                                                       # and the next call is none the worse
+
+
+def test_tensors_that_want_a_gradient_are_refused(bk, cuda):
+    w = World(bk, cuda, [40, 20], [1, 1], H=2, Hq=4, seed=72, ragged=False)
+    k, q = w.randn(2).to(cuda), w.randn(4).to(cuda)
+    wants = lambda x: x.clone().requires_grad_()
+    for bad in (lambda: w.cache.attend(1, wants(q), w.table_d, w.lens_d), lambda: w.cache.append(1, wants(k), k, w.table_d, w.lens_d),
+                lambda: w.cache.append(1, k, wants(k), w.table_d, w.lens_d), lambda: w.cache.attend(1, q, w.table_d, w.lens_d, out=wants(q))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            bad()
+    with torch.no_grad():
+        w.cache.append(1, wants(k), k, w.table_d, w.lens_d)
+        w.cache.attend(1, wants(q), w.table_d, w.lens_d)
+    w.cache.check()
+
+
 def test_the_softmax_scale_and_peaked_rows(bk, cuda):
     for scale in (0.0, -0.3, 0.02, 2.0):
         w = World(bk, cuda, [300, 77], [1, 4], H=2, Hq=8, seed=20)
