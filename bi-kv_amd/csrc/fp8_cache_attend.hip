@@ -23,6 +23,10 @@ namespace bikv {
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr int kNoKey = 0x7fffffff;      // position of a key that no row sees
 constexpr int kPShift = 8;              // p is scaled by 2^8 in fp16: p down to 2^-22 stays normal
+// z is taken against a row's last reference m, which moves only when some z exceeds it by more than this: p may be up to 2^4, p
+// 2^kPShift vs 2^-r < 2^(4 + 8 + 1) is in fp16's range, and most steps rescale nothing and reduce nothing across lanes. With 0,
+// chunks of 900 behind 8192 tokens take 704 us where they take 682 with 4.
+constexpr float kSlack = 4.f;
 
 template <int TYPE> struct QType;
 template <> struct QType<0> { typedef bf16x8 V8; };
@@ -404,7 +408,16 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
       const bool edge = (step + 1) * kKeys > all || __ballot(pos == kNoKey) != 0;
 
       __builtin_amdgcn_sched_barrier(0);
-      // S^T = K Q^T
+      // S^T = K Q^T; what it needs from LDS is asked for at once, not piece by piece with a wait for each
+      u32x4 kx[NK][D / 64];
+      f32x4 ks[NK], vs[NK];
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) kx[i][j] = meta.kv[0][(16 * i + col) * kChunks + ((4 * j + quad) ^ swizzle(16 * i + col))];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) ks[i] = *reinterpret_cast<const f32x4*>(&meta.ks[16 * i + 4 * quad]);
+      __builtin_amdgcn_sched_barrier(0);
       f32x4 s[NT][NK];
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
@@ -413,10 +426,9 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
           u32x4 f[2];
-          const u32x4 x = meta.kv[0][(16 * i + col) * kChunks + ((4 * j + quad) ^ swizzle(16 * i + col))];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const u32x2 lo = widen4<TYPE>(x[2 * half]), hi = widen4<TYPE>(x[2 * half + 1]);
+            const u32x2 lo = widen4<TYPE>(kx[i][j][2 * half]), hi = widen4<TYPE>(kx[i][j][2 * half + 1]);
             f[half] = u32x4{lo[0], lo[1], hi[0], hi[1]};
           }
 #pragma unroll
@@ -426,6 +438,8 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < NK; ++i) vs[i] = *reinterpret_cast<const f32x4*>(&meta.vs[16 * i + 4 * quad]);
       __builtin_amdgcn_sched_barrier(0);
       int next = kNoKey;
       if (more) {
@@ -441,11 +455,9 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         uint32_t hidden = 0;                     // bit per key of the lane: the row does not see it
         float top = kMinusInf;
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const f32x4 ks = *reinterpret_cast<const f32x4*>(&meta.ks[16 * i + 4 * quad]);
+        for (int i = 0; i < NK; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[t][i][c] *= ks[c];
-        }
+          for (int c = 0; c < 4; ++c) s[t][i][c] *= ks[i][c];
         if (edge) {
 #pragma unroll
           for (int i = 0; i < NK; ++i)
@@ -460,9 +472,9 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) top = fmaxf(top, s[t][i][c]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__ballot(top > m[t])) {
+        if (__ballot(top > m[t] + kSlack)) {
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
           const float now = fmaxf(m[t], top);
           const float grow = now == kMinusInf ? 1.f : exp2_fast(m[t] - now);       // 0 at the first key
           m[t] = now;
@@ -474,15 +486,13 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         }
         const float from = m[t] == kMinusInf ? 0.f : m[t];
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const f32x4 vs = *reinterpret_cast<const f32x4*>(&meta.vs[16 * i + 4 * quad]);
+        for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float e = exp2_fast(s[t][i][c] - from);
             l[t] += e;
-            s[t][i][c] = e * vs[c];
+            s[t][i][c] = e * vs[i][c];
           }
-        }
         if (edge) {                              // 0 times a scale that is not finite
 #pragma unroll
           for (int i = 0; i < NK; ++i)
@@ -801,7 +811,6 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
-constexpr float kSlack = 4.f;           // p 2^kPShift vs 2^-r < 2^(4 + 8 + 1), in fp16's range; with 0, chunks of 900 behind 8192 tokens take 704 us, with 4 682
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -1046,9 +1055,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       kf[j] = at_k(buf, (k_at ^ (32 * j)) + 32 * kKRow);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // The lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4. z is taken against the row's last reference m, which is
-    // moved only when some z exceeds it by kSlack: p may then be up to 2^kSlack, which fp16 has room for, and most steps
-    // rescale nothing and reduce nothing across lanes.
+    // The lane's keys: 32 kb + 8 (i / 4) + 4 half + i % 4.
     const float from = m_run == kMinusInf ? 0.f : m_run;
     float top = kMinusInf;
     auto take_z = [&](int kb) {
