@@ -113,13 +113,15 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 //
 // Two ways of cutting the work, chosen by the host: every tile a workgroup of its own (no second launch), or, where sequences
 // may be long, even shares: the tiles of all sequences times their key steps form one line, share s of which is slot s's.
+// A tile's steps have a few steps' room before them, which stands for what beginning a tile costs a workgroup.
 // A tile that lies in one share is finished there; of the others each share leaves (O, m, l), and
 // fp8_join_few_kernel joins them.
 // ---------------------------------------------------------------------------------------------
+constexpr int kFewWaves = 8;               // of 256 registers: they fill a CU
 template <int D, int TYPE, int NT, int NK>
 struct Few {
   static constexpr int kM = 16 * NT;       // rows of a tile
-  static constexpr int kWaves = 8;         // of 256 registers: they fill a CU
+  static constexpr int kWaves = kFewWaves;
   static constexpr int kKeys = 16 * NK;    // keys of a step
   static constexpr int kDT = D / 16;       // bytes of a V row per lane, and row tiles of O^T
   static constexpr int kChunks = D / 16;   // 16-byte pieces of a key's row
@@ -157,7 +159,7 @@ __device__ __forceinline__ uint32_t weight_of(const AttendArgs& a, int64_t b) {
   if (b >= a.seq.n_seqs) return 0;
   const Seq s = read_seq(a.seq, b);
   if (!s.ok) raise_flag(a.status, ST_SLOT_SRC);
-  return tiles_of(s, a.group, M) * steps_of(s, KEYS);
+  return tiles_of(s, a.group, M) * (steps_of(s, KEYS) + (uint32_t)a.begin_cost);
 }
 
 // The number of the row tile that sequence b's first row begins: with one token each the sequences have as many tiles
@@ -261,7 +263,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
     const int64_t tile = slot - first_tile<kM>(a, b);
     if (!seq.ok || tile < 0 || tile >= (int64_t)tiles_of(seq, a.group, kM)) return;
     const uint32_t steps = (uint32_t)uni((int)steps_of(seq, kKeys));
-    local = (uint32_t)uni((int)tile) * steps;
+    local = (uint32_t)uni((int)tile) * steps;                    // the host sets begin_cost to 0
     line = {steps, 0, steps};
   }
 
@@ -272,23 +274,28 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
       seq_of = b;
     }
     const int steps = uni((int)steps_of(seq, kKeys));
-    const uint32_t weight = (uint32_t)uni((int)(tiles_of(seq, a.group, kM) * (uint32_t)steps));
+    // a tile's place on the line: its begin_cost, then its steps
+    const int room = steps + a.begin_cost;
+    const uint32_t weight = (uint32_t)uni((int)(tiles_of(seq, a.group, kM) * (uint32_t)room));
     if (local >= weight) {
       ++b;
       local = 0;
       continue;
     }
-    const int tile = (int)(local / (uint32_t)steps);
-    const int step0 = (int)local - tile * steps;
-    int count = steps - step0;
-    if ((uint32_t)count > line.end - at) count = (int)(line.end - at);
+    const int tile = (int)(local / (uint32_t)room);
+    const int x0 = (int)local - tile * room;
+    int taken = room - x0;
+    if ((uint32_t)taken > line.end - at) taken = (int)(line.end - at);
+    const int step0 = x0 > a.begin_cost ? x0 - a.begin_cost : 0;
+    const int count = x0 + taken - a.begin_cost - step0;
+    if (count <= 0) break;                                       // the share ends before the tile's steps begin: the next one has them all
     const bool first_of_share = at == line.begin;
     const bool whole = count == steps;
     const int rows = uni((int)((int64_t)seq.n * G - (int64_t)tile * kM < kM ? (int64_t)seq.n * G - (int64_t)tile * kM : kM));
     const int len = uni(seq.len);
     const int before = a.causal ? uni(seq.len - seq.n) : 0;     // keys older than the call's own (negative: some rows see none)
     if (step0 == 0 && !whole) {
-      int parts = (int)((at + steps - 1) / line.per) - slot + 1;
+      int parts = (int)((at + (room - x0) - 1) / line.per) - slot + 1;
       if (parts > a.slots - slot) parts = a.slots - slot;          // row numbers that make no sense may have wrapped the line's length
       join = {seq.first, tile, rows, parts, 2 * slot + (first_of_share ? 0 : 1)};
     }
@@ -709,8 +716,8 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         lds_barrier();                                             // before the space is written again
       }
     }
-    at += count;
-    local += count;
+    at += taken;
+    local += taken;
   }
   if (a.slots > 1 && h0 == 0 && tid == 0) a.part_join[slot] = join;
 }
@@ -1315,11 +1322,11 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
   // against 141; a 64-row tile of this kind was 2 to 3 times slower than the many rows' and is not there.
   const int m = mean <= 16 ? 16 : 32, keys = m == 16 ? 64 : 32;
   const int64_t tiles = tiles_in_all(one_each, group, n_seqs, n_rows, m);
-  if (mean <= 32 && tiles * ((max_len + keys - 1) / keys + 1) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
+  if (mean <= 32 && tiles * ((max_len + keys - 1) / keys + 1 + 2 * kFewWaves) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
     p.form = m == 16 ? ATTEND_FEW_16 : ATTEND_FEW_32;
     p.rows = m;
     p.tiles = tiles;
-    const int waves = 8;
+    const int waves = kFewWaves;
     p.heads_per_group = heads < waves ? heads : waves;
     if (max_len <= 1024) {
       // A workgroup per tile, no second launch: 11.5 us against 16 for a sequence of 500 tokens, 15 against 16 at 1000; at 1500
@@ -1335,6 +1342,9 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
       p.slots = (int32_t)(slots < 1 ? 1 : slots);
     }
     p.min_steps = waves / p.heads_per_group;
+    // 3 steps of each wave of a head: 64 sequences of 100 to 4000 tokens, 3 new each, 28 and 4 heads, take 51 us, 64 without and 59
+    // with one; 64 of 1k to 8k, 64 and 8 heads, 140, 148 and 144.
+    p.begin_cost = p.slots > 0 ? 3 * p.min_steps : 0;
     p.part_rows = p.slots > 1 ? 2 * (int64_t)p.slots * heads * p.rows : 0;
   } else {
     p.form = ATTEND_MANY;
@@ -1388,6 +1398,7 @@ hipError_t launch_fp8_attend(const AttendPlan& p, int head_dim, int type, const 
   AttendArgs a = args;
   a.slots = p.slots;
   a.min_steps = p.min_steps;
+  a.begin_cost = p.begin_cost;
   a.tiles = p.tiles;
   a.heads_per_group = p.heads_per_group;
   if (head_dim == 128) return type == 0 ? launch_form<128, 0>(p, a, stream) : launch_form<128, 1>(p, a, stream);

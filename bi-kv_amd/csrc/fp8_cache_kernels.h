@@ -71,6 +71,7 @@ struct AttendArgs {
   JoinHead* part_join;       // few rows: one per slot
   int32_t slots;             // few rows: shares the work is cut into, 0 = a workgroup per tile; many rows: parts a tile's keys are cut into
   int32_t min_steps;         // few rows: key steps a share has at least
+  int32_t begin_cost;        // few rows: steps' worth of room before a tile's steps
   int32_t heads_per_group;   // few rows: KV heads of a workgroup
   int64_t tiles;             // row tiles of the launch
   uint32_t* status;
@@ -81,6 +82,7 @@ struct AttendPlan {
   int rows;                  // rows of a tile
   int32_t slots;
   int32_t min_steps;
+  int32_t begin_cost;
   int32_t heads_per_group;
   int64_t tiles;
   int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
