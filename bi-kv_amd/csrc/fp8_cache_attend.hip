@@ -98,9 +98,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // heads; where there are more waves than heads, several waves share a head and take its steps in turn.
 //
 // Measured, with fp8_join_few_kernel: 64 sequences of 1024 to 8192 tokens, 64 query and 8 KV heads of 128, bf16, one new token
-// each: 612 MB in 121 + 7 us, 5.05 TB/s while the first kernel runs; 3 of 32k, 32 heads: 186 MB in 37 + 8 us; 24 of up to 5000
-// with up to 5 new tokens, 28 and 4 heads: 69 MB in 34 + 6 us; one of 777, 12 and 2 heads: 13.5 us, where what counts is the
-// chain of lookups (lengths, page ids, scales and rows) and how long code and data take to arrive.
+// each: 612 MB in 118 + 7 us, 5.2 TB/s while the first kernel runs; 3 of 32k, 32 heads: 186 MB in 37 + 8 us; 24 of up to 5000
+// with up to 5 new tokens, 28 and 4 heads: 69 MB in 30 + 6 us, some 1.4 us of instructions to a step of a 32-row tile, whose
+// loads are no longer what it waits for (twice the buffers changed nothing); one of 777, 12 and 2 heads: 12.5 us, where what counts
+// is the chain of lookups (lengths, page ids, scales and rows) and how long code and data take to arrive.
 //
 // Bound by memory: every byte of K and V is read once per row tile. Each wave copies its own steps' rows into its own part
 // of LDS (global_load_lds, 16 bytes a lane, whole rows) and never waits for another wave while it goes: scales and the next
@@ -795,8 +796,8 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // Many rows per sequence: a workgroup of four waves does 128 rows of one KV head, 32 a wave, over the
 // keys 64 at a time.
 //
-// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 242 us (568 TFLOP/s); 6 chunks of
-// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 750 us (741 TFLOP/s); 5 of up to 700 tokens and
+// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 244 us (563 TFLOP/s); 6 chunks of
+// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 751 us (740 TFLOP/s); 5 of up to 700 tokens and
 // 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 39 us.
 //
 // Bound by what the matrix products (4 D flops per visible row and key), the softmax beside them (an exp2 and some six other
