@@ -63,10 +63,8 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-typedef __attribute__((ext_vector_type(2))) short s16x2;
-typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // Four values, two to a word as they were read, divided by a power of two and rounded to the nearest e4m3.
 template <int TYPE>
@@ -218,7 +216,9 @@ __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
         const int r = c * kChunk + i * kRows + sub;
-        if (r < n) gstore<u32x2>(page + (uint64_t)((r0 + r) * a.layer.token_stride), u32x2{pack4_scaled<TYPE>(x[i][0], x[i][1], scale), pack4_scaled<TYPE>(x[i][2], x[i][3], scale)});
+        if (r < n)
+          gstore<u32x2>(page + (uint64_t)((r0 + r) * a.layer.token_stride),
+                        u32x2{pack4_scaled<TYPE>(x[i][0], x[i][1], scale), pack4_scaled<TYPE>(x[i][2], x[i][3], scale)});
       }
       continue;
     }
