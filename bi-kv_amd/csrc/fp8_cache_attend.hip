@@ -1355,13 +1355,13 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
     // steps, and some two steps more to begin and to end (two again where empty workgroups, of tiles that sequences may have
     // and these do not, take a place first); the parts' sums are written and read again, 115 of them in a step's time. 33 sequences of 40 to 64 rows over 4000 keys, 8 KV heads: 243 us in one part, 184 in three; 300 new
     // tokens of each of 2 sequences of 3500, 4 KV heads: 52 us in 6 parts, 119 in one and 66 in 12. From 1024 tiles on the rounds
-    // even out by themselves. Parts have four steps at least.
+    // even out by themselves. Parts have four steps at least, and their sums take 140 MB at most.
     const int64_t tiles_likely = one_each ? p.tiles : all / kManyRows + n_seqs / 2, n = heads * (tiles_likely > n_seqs ? tiles_likely : n_seqs);
     const int64_t steps = (max_len + kManyKeys - 1) / kManyKeys;
     p.slots = 1;
     if (n < 1024) {
       int64_t least = -1;
-      for (int64_t parts = 1; parts <= 64 && (parts == 1 || parts <= steps / 4); ++parts) {
+      for (int64_t parts = 1; parts <= 64 && (parts == 1 || (parts <= steps / 4 && p.tiles * heads * parts <= 2048)); ++parts) {
         const int64_t cost = (n * parts + 511) / 512 * ((steps + parts - 1) / parts + 2) + (parts > 1 ? n * parts / 115 + 2 : 0) + (p.tiles * heads * parts > 512 ? 2 : 0);
         if (least < 0 || cost < least) {
           least = cost;
