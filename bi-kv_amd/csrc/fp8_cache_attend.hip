@@ -1275,7 +1275,9 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   }
 }
 
-// Joins the parts of a tile's keys: D/4 threads a row, each with four places over all parts, of which there are few.
+constexpr int kMostParts = 64;
+// Joins the parts of a tile's keys: D/4 threads a row, each with a share of the parts' (m, l) and four places over all parts, four
+// parts' places under way at a time.
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) {
   constexpr int kRows = 256 / (D / 4);            // rows of a workgroup
@@ -1292,20 +1294,46 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
   if (!seq.ok || tile < 0 || tile * kManyRows + r >= (int64_t)seq.n * G) return;
   const uint32_t row = (uint32_t)(tile * kManyRows + r), tok = divide(row, a.group);
   auto at = [&](int i) { return ((slot * H + h) * a.slots + i) * kManyRows + r; };
-  float top = kMinusInf;
-  for (int i = 0; i < a.slots; ++i) top = fmaxf(top, a.part_ml[2 * at(i)]);
+  constexpr int kLanes = D / 4, kMine = kMostParts / kLanes;
+  const int mine = threadIdx.x % kLanes, first_lane = lane - mine;
+  float w[kMine], l[kMine], top = kMinusInf;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int i = k * kLanes + mine;
+    w[k] = kMinusInf;
+    l[k] = 0.f;
+    if (i < a.slots) {
+      w[k] = a.part_ml[2 * at(i)];
+      l[k] = a.part_ml[2 * at(i) + 1];
+    }
+    top = fmaxf(top, w[k]);
+  }
+#pragma unroll
+  for (int k = 1; k < kLanes; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
   const float from = top == kMinusInf ? 0.f : top;
   f32x4 o = {0, 0, 0, 0};
   float sum = 0.f;
-  for (int i = 0; i < a.slots; ++i) {
-    float w = a.part_ml[2 * at(i) + 1];
-    if (w == 0.f) continue;                       // saw no key: what it holds was never written
-    w *= exp2_fast(a.part_ml[2 * at(i)] - from);
-    const f32x4 y = gload<f32x4>((uint64_t)(a.part_o + at(i) * D + d));
-    sum += w;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] += w * y[c];
+  for (int k = 0; k < kMine; ++k) {
+    w[k] = l[k] == 0.f ? 0.f : l[k] * exp2_fast(w[k] - from);
+    sum += w[k];
   }
+#pragma unroll
+  for (int k = 1; k < kLanes; k <<= 1) sum += __shfl_xor(sum, k);
+#pragma unroll
+  for (int k = 0; k < kMine; ++k)
+    for (int i0 = k * kLanes; i0 < (k + 1) * kLanes && i0 < a.slots; i0 += 4) {
+      f32x4 y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = gload<f32x4>((uint64_t)(a.part_o + at(i0 + u < a.slots ? i0 + u : a.slots - 1) * D + d));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float wi = __shfl(w[k], first_lane + i0 + u - k * kLanes);
+        if (i0 + u < a.slots && wi != 0.f)        // what a part that saw no key holds was never written
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] += wi * y[u][c];
+      }
+    }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int head = h * G + (int)(row - tok * G);
   gstore<u32x2>((uint64_t)a.out + 2 * ((seq.first + tok) * a.o_row + head * a.o_head + d),
@@ -1361,7 +1389,7 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
     p.slots = 1;
     if (n < 1024) {
       int64_t least = -1;
-      for (int64_t parts = 1; parts <= 64 && (parts == 1 || (parts <= steps / 4 && p.tiles * heads * parts <= 2048)); ++parts) {
+      for (int64_t parts = 1; parts <= kMostParts && (parts == 1 || (parts <= steps / 4 && p.tiles * heads * parts <= 2048)); ++parts) {
         const int64_t cost = (n * parts + 511) / 512 * ((steps + parts - 1) / parts + 2) + (parts > 1 ? n * parts / 115 + 2 : 0) + (p.tiles * heads * parts > 512 ? 2 : 0);
         if (least < 0 || cost < least) {
           least = cost;
