@@ -1346,12 +1346,13 @@ AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, 
   AttendPlan p = {};
   const int64_t all = n_rows * group;                      // rows of one KV head
   const int64_t mean = (all + n_seqs - 1) / n_seqs;
-  // Few rows: the fewer, the more of a wide tile would be computed for nothing. Rows of a sequence on average, 64 sequences of
-  // 3500 tokens, 8 KV heads: 16 rows 113 us against 137 as many rows; 28 rows (4 heads) 75 against 116; 32 rows 144
-  // against 141; a 64-row tile of this kind was 2 to 3 times slower than the many rows' and is not there.
+  // Up to 16 rows of a sequence on average: few rows (3 sequences of 32k, 8 KV heads, 16 rows: 58 us against 69 as many rows; 64 of
+  // 3000: 113 and 137). Up to 32: where the sequences are many enough for the shares (64 of 3000, 21 rows, 4 heads, 63 us against
+  // 119; 12 of 4500, 33 and 35; but 6 of 3000, 27 and 23; one of 20000, 43 and 30). More: many rows; a 64-row tile of the first
+  // kind took two to three times as long.
   const int m = mean <= 16 ? 16 : 32, keys = m == 16 ? 64 : 32;
   const int64_t tiles = tiles_in_all(one_each, group, n_seqs, n_rows, m);
-  if (mean <= 32 && tiles * ((max_len + keys - 1) / keys + 1 + 2 * kFewWaves) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
+  if ((mean <= 16 || (mean <= 32 && n_seqs >= 8)) && tiles * ((max_len + keys - 1) / keys + 1 + 2 * kFewWaves) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
     p.form = m == 16 ? ATTEND_FEW_16 : ATTEND_FEW_32;
     p.rows = m;
     p.tiles = tiles;

@@ -366,6 +366,10 @@ SHAPES = [
     ([200, 77], [2, 3], 17, 5, 64),
     ([40] * 53, [1 + i % 2 for i in range(53)], 4, 8, 128),          # as many workgroups as CUs, and more
     ([30 + i for i in range(130)], None, 3, 6, 64),
+    ([90 + 41 * i for i in range(10)], [5 - i % 5 for i in range(10)], 2, 7, 128),        # 7 to 35 rows, eight sequences and more
+    ([20 + 50 * i for i in range(9)], None, 3, 32, 64),
+    ([700 - 60 * i for i in range(10)], [2 + i % 2 for i in range(10)], 9, 8, 64),
+    ([1500, 3, 0, 800, 64, 65, 1, 31], [4, 3, 0, 4, 4, 1, 1, 5], 2, 8, 128),
     ([1024, 1000], None, 2, 4, 128), ([1025, 17], None, 2, 4, 128),  # either side of the length from which work is cut
 ]
 
