@@ -173,7 +173,7 @@ __device__ __forceinline__ int64_t first_tile(const AttendArgs& a, int64_t b) {
   return q * a.group.d / M + b;
 }
 static int64_t tiles_in_all(bool one_each, int group, int64_t n_seqs, int64_t n_rows, int m) {
-  return one_each ? n_seqs * ((group + m - 1) / m) : n_rows * group / m + n_seqs;
+  return one_each ? n_seqs * (((int64_t)group + m - 1) / m) : n_rows * group / m + n_seqs;
 }
 
 // The line's length (the host sees to it that it stays below 2^31).
