@@ -28,10 +28,6 @@ constexpr int kPShift = 8;              // p is scaled by 2^8 in fp16: p down to
 // chunks of 900 behind 8192 tokens take 704 us where they take 682 with 4.
 constexpr float kSlack = 4.f;
 
-template <int TYPE> struct QType;
-template <> struct QType<0> { typedef bf16x8 V8; };
-template <> struct QType<1> { typedef f16x8 V8; };
-
 // Four e4m3 bytes as two pairs of q's type.
 template <int TYPE>
 __device__ __forceinline__ u32x2 widen4(uint32_t c) {
