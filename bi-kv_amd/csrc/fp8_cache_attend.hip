@@ -11,11 +11,15 @@
 // S^T = K Q^T and O^T = V^T P^T. A lane of S^T then holds a few keys of ONE row, which is the layout the second product
 // takes its P^T operand in, as long as V^T's keys are put in the same order: P never crosses lanes or
 // memory. K is widened to q's type and Q K^T is exact up to fp32 sums. P is rounded to fp16 (11 bits; bf16's 8 would
-// cost as much as the output's own rounding): p vs 2^(8 - r) with r the largest exponent of vs so far, so that
-// neither a page's scale nor a small p leaves fp16's range; the exponent comes off again at the end. Where q is fp16, 11 bits
-// would cost as much as the output's own rounding, and P goes as the sum of two fp16 numbers. A page whose V scale is
-// below 2^-22 of the largest among the keys read before it loses bits against that page's values, not against the larger ones.
-// l sums the unrounded p.
+// cost as much as the output's own rounding): p vs 2^(8 - r), so that neither a page's scale nor a small p leaves fp16's range; the
+// exponent r comes off again at the end. Where q is fp16, 11 bits would cost as much as the output's own rounding, and P goes as
+// the sum of two fp16 numbers. l sums the unrounded p.
+//
+// r: while the V scales of the keys read so far lie within 2^kSpread of each other, the largest one's exponent, the same for all rows of
+// a tile. A row's largest p vs 2^(8 - r) is then 1 at least, whichever of these keys the row sees: a weight p vs keeps its bits
+// down to 2^-14 of the row's largest one, and is off by 2^-25 of that at most below. Once they lie farther apart each
+// row has an r of its own, that of the largest p vs among the keys it does see ("wide" steps, to the end of the tile): a page that a row
+// does not see, or hardly attends to, takes no bits from the pages it does. They cost few rows 3 to 8 %, many rows a third.
 #include "fp8_cache_device.h"
 
 namespace bikv {
@@ -27,6 +31,8 @@ constexpr int kPShift = 8;              // p is scaled by 2^8 in fp16: p down to
 // 2^kPShift vs 2^-r < 2^(4 + 8 + 1) is in fp16's range, and most steps rescale nothing and reduce nothing across lanes. With 0,
 // chunks of 900 behind 8192 tokens take 704 us where they take 682 with 4.
 constexpr float kSlack = 4.f;
+constexpr int kSpread = 8;
+constexpr int kLeastR = -400;           // below any exponent that is left over in a sum
 
 // Four e4m3 bytes as two pairs of q's type.
 template <int TYPE>
@@ -86,8 +92,28 @@ __device__ __forceinline__ int scale_exponent(float s) {
   const int e = (int)((__float_as_uint(s) >> 23) & 0xffu);
   return e == 0 || e == 255 ? -126 : e - 127;
 }
+__device__ __forceinline__ bool scale_is_finite(float s) { return (__float_as_uint(s) & 0x7f800000u) != 0x7f800000u; }
+// The largest and the smallest exponent among the lanes' scales, -126 and 127 from lanes without one or with one that is not
+// finite (it spoils the rows that see it, and has no say in the others').
+struct Exponents { int top, low; };
+__device__ __forceinline__ Exponents exponents_of(bool there, float s) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const short e = (short)scale_exponent(s);
+  s16x2 most{there ? e : (short)-126, (short)(there && scale_is_finite(s) ? -e : -127)};       // both in one word: half the exchanges
+  for (int k = 32; k > 0; k >>= 1) most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, __shfl_xor(__builtin_bit_cast(int, most), k)));
+  return {uni(most[0]), uni(-most[1])};
+}
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Wide steps: vs = mantissa * 2^exponent, the mantissa less than 1. A scale that is zero or not finite has the exponent -inf.
+__device__ __forceinline__ float wide_exponent(float vs) { return vs != 0.f && scale_is_finite(vs) ? (float)__builtin_amdgcn_frexp_expf(vs) : kMinusInf; }
+__device__ __forceinline__ float wide_mantissa(float vs) { return __builtin_amdgcn_frexp_mantf(vs); }
+// A row's r after a step whose largest weight is below 2^top and in which the row's reference moved up by `moved`.
+__device__ __forceinline__ int row_exponent(int r, float moved, float top) {
+  const int older = r - (int)fminf(moved, 1000.f), now = (int)ceilf(fmaxf(top, (float)kLeastR)), y = older > now ? older : now;
+  return y > kLeastR ? y : kLeastR;
+}
 
 // ---------------------------------------------------------------------------------------------
 // Few rows per sequence: a workgroup takes a tile of 16 or 32 rows over a run of key steps, its waves the KV
@@ -215,8 +241,10 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
     float ks_in[64], vs_in[64];            // the copies' targets: a step's scales, the next step's page ids
     uint32_t pid_in[2][64];
     float ks[kKeys], vs[kKeys];
+    float ex[kKeys];                       // wide steps: the exponents of the V scales, whose mantissas are in vs
     int pos[kKeys];
     int nan_at[D];                         // by place: the first key with a NaN in V that not every row sees
+    int r[kM];                             // wide steps: the rows' r
   };
   __shared__ Meta metas[kWaves];
   __shared__ float sums[kWaves][2][kM];    // the waves' m and l
@@ -374,8 +402,8 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
 
     f32x4 o[NT][kDT];
     float m[NT], l[NT];
-    int r_exp = -126;
-    bool spoilt = false;
+    int r_exp = -126, r_low = 127;         // exponents of the V scales read so far
+    bool wide = false, spoilt = false;
     for (int d = lane; d < D; d += 64) meta.nan_at[d] = kNoKey;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -388,25 +416,26 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
     auto compute = [&](int step, int which, int pos, bool more) {
       wait_vmem<kCopies>();                                      // all but V
       const float ks_in = meta.ks_in[lane], vs_in = meta.vs_in[lane];
-      // a larger V scale than any before: what is summed moves to its exponent
+      // a larger V scale than any before: what is summed moves to its exponent, or the steps are wide from here on
       const int e = pos != kNoKey ? scale_exponent(vs_in) : -126;
-      if (__ballot(e > r_exp)) {
-        int top = e;
-        for (int k = 32; k > 0; k >>= 1) {
-          const int y = __shfl_xor(top, k);
-          top = y > top ? y : top;
-        }
-        top = uni(top);
+      if (!wide && __ballot(e > r_exp || (e < r_low && pos != kNoKey && scale_is_finite(vs_in)))) {
+        const Exponents now = exponents_of(pos != kNoKey, vs_in);
+        const int top = now.top > r_exp ? now.top : r_exp;
+        r_low = now.low < r_low ? now.low : r_low;
+        wide = top - r_low > kSpread;
+        if (wide && lane < kM) meta.r[lane] = r_exp;
+        const int by = wide ? 0 : r_exp - top;                   // no branch: in two ways the sums would be held twice
+        r_exp = wide ? r_exp : top;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < kDT; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[t][i][c] = ldexpf(o[t][i][c], r_exp - top);
-        r_exp = top;
+            for (int c = 0; c < 4; ++c) o[t][i][c] = ldexpf(o[t][i][c], by);
       }
       meta.ks[lane & (kKeys - 1)] = ks_in * a.scale_log2;
-      meta.vs[lane & (kKeys - 1)] = ldexpf(vs_in, kPShift - r_exp);
+      meta.vs[lane & (kKeys - 1)] = wide ? wide_mantissa(vs_in) : ldexpf(vs_in, kPShift - r_exp);
+      if (wide) meta.ex[lane & (kKeys - 1)] = wide_exponent(vs_in);
       meta.pos[lane & (kKeys - 1)] = pos;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       const bool edge = (step + 1) * kKeys > all || __ballot(pos == kNoKey) != 0;
@@ -453,6 +482,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
       }
       __builtin_amdgcn_sched_barrier(0);
       // softmax: the lane's keys are 16 i + 4 quad + c
+      const float counted = wide ? 0.f : 1.f;
       u32x4 p[NT][NK / 2], p_low[NT][TYPE == 1 ? NK / 2 : 1];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -476,25 +506,54 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) top = fmaxf(top, s[t][i][c]);
-        if (__ballot(top > m[t] + kSlack)) {
+        if (wide || __ballot(top > m[t] + kSlack)) {
           top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32));
           const float now = fmaxf(m[t], top);
           const float grow = now == kMinusInf ? 1.f : exp2_fast(m[t] - now);       // 0 at the first key
+          const float moved = now == m[t] ? 0.f : now - m[t];
           m[t] = now;
           l[t] *= grow;
 #pragma unroll
           for (int i = 0; i < kDT; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[t][i][c] *= grow;
+          if (wide) {                              // l by itself; z then takes the scale's exponent along, relative to the row's r
+            float most = kMinusInf;
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+              const f32x4 ex = *reinterpret_cast<const f32x4*>(&meta.ex[16 * i + 4 * quad]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                s[t][i][c] -= m[t] == kMinusInf ? 0.f : m[t];
+                l[t] += exp2_fast(s[t][i][c]);
+                most = fmaxf(most, s[t][i][c] + ex[c]);
+              }
+            }
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const int was = meta.r[16 * t + col], r = row_exponent(was, moved, most);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            meta.r[16 * t + col] = r;
+#pragma unroll
+            for (int i = 0; i < kDT; ++i)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[t][i][c] = ldexpf(o[t][i][c], was - r);
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+              const f32x4 ex = *reinterpret_cast<const f32x4*>(&meta.ex[16 * i + 4 * quad]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s[t][i][c] += ex[c] + (float)(kPShift - r);
+            }
+          }
         }
-        const float from = m[t] == kMinusInf ? 0.f : m[t];
+        const float from = wide || m[t] == kMinusInf ? 0.f : m[t];
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float e = exp2_fast(s[t][i][c] - from);
-            l[t] += e;
+            l[t] = fmaf(e, counted, l[t]);
             s[t][i][c] = e * vs[i][c];
           }
         if (edge) {                              // 0 times a scale that is not finite
@@ -613,6 +672,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
       l[t] += __shfl_xor(l[t], 16);
       l[t] += __shfl_xor(l[t], 32);
     }
+    auto r_of = [&](int t) { return (wide ? meta.r[16 * t + col] : r_exp) - kPShift; };    // what comes off the row's sums
     const int64_t part0 = ((int64_t)(2 * slot + (first_of_share ? 0 : 1)) * H) * kM;       // the segment's place among the parts
     // What is known of a row once all of its keys in the segment are: its lse, or its (m, l)
     auto leave_sum = [&](int r, uint32_t token, int hd, float top, float sum) {
@@ -630,6 +690,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
         for (int t = 0; t < NT; ++t) {
           if (!live[t]) continue;
           const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
+          const int off = r_of(t);
           if (quad == 0) leave_sum(16 * t + col, tok[t], head[t], m[t], l[t]);
           const uint64_t dst = whole ? (uint64_t)a.out + 2 * ((seq.first + tok[t]) * a.o_row + head[t] * a.o_head)
                                      : (uint64_t)(a.part_o + (part0 + (int64_t)h * kM + 16 * t + col) * D);
@@ -637,7 +698,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
           for (int c = 0; c < 4; ++c) {
             float y[kDT];
 #pragma unroll
-            for (int dt = 0; dt < kDT; ++dt) y[dt] = ldexpf(o[t][dt][c] * inv, r_exp - kPShift);
+            for (int dt = 0; dt < kDT; ++dt) y[dt] = ldexpf(o[t][dt][c] * inv, off);
             const int d = kDT * (4 * quad + c);
             if (whole) {
               if constexpr (kDT == 8)
@@ -678,6 +739,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) sum += li[i] == 0.f ? 0.f : li[i] * exp2_fast(mi[i] - from);
         const float mine = l[t] == 0.f ? 0.f : exp2_fast(m[t] - from) / sum;
+        const int off = r_of(t);
         float* space = reinterpret_cast<float*>(meta.kv);            // 16 rows of D floats
         // a row's 16-byte pieces are XOR-ed with its number: sixteen lanes write sixteen rows at one place
 #pragma unroll
@@ -686,7 +748,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
           for (int dt = 0; dt < kDT; dt += 4) {
             f32x4 y;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = ldexpf(o[t][dt + k][c] * mine, r_exp - kPShift);
+            for (int k = 0; k < 4; ++k) y[k] = ldexpf(o[t][dt + k][c] * mine, off);
             *reinterpret_cast<f32x4*>(space + col * D + 4 * (((kDT * (4 * quad + c) + dt) / 4) ^ (col & (D / 4 - 1)))) = y;
           }
         if (works && way == 0 && quad == 0 && live[t]) leave_sum(r, tok[t], head[t], top, sum);
@@ -815,6 +877,7 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
+constexpr int kWide = 1 << 20;          // in r's place: the step is a wide one
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -833,12 +896,15 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   struct Meta {
     uint64_t off[kKeys];
     float ks[kKeys], vs[kKeys];                   // as they are in the cache; then times the softmax's scale and log2(e), and times 2^(kPShift - r)
+    float ex[kKeys];                              // wide steps: the exponents of the V scales, whose mantissas are in vs then
     int pos[kKeys];
-    int gone, e, r;                               // some key is nobody's; the largest exponent of V's scales here; and up to here
+    int gone, r;                                  // some key is nobody's; the largest exponent of V's scales up to here, or kWide
+    Exponents e;                                  // of V's scales here
   };
   __shared__ uint32_t pids_in[4][2][kKeys];       // page ids of the keys to be looked up next, low and high words
   __shared__ int nan_at[D];                       // by place: the first key with a NaN in V that not every row sees
   __shared__ int spoilt;
+  __shared__ int row_r[kManyRows];                // wide steps: the rows' r
   __shared__ u32x4 k_lds[2][kKeys * kChunks];
   __shared__ u32x4 v_lds[2][D * 8];
   __shared__ Meta metas[8];
@@ -932,24 +998,24 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     copy4_to_lds((uint64_t)a.layer.ks + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.ks)));
     copy4_to_lds((uint64_t)a.layer.vs + 4 * h + (uint64_t)(page * a.layer.scale_stride), (uint32_t)uni((int)lds_address(m.vs)));
   };
-  auto find_exponent = [&](Meta& m) {
-    int e = m.pos[lane] != kNoKey ? scale_exponent(m.vs[lane]) : -126;
-    for (int i = 32; i > 0; i >>= 1) {
-      const int y = __shfl_xor(e, i);
-      e = y > e ? y : e;
-    }
+  auto find_exponents = [&](Meta& m) {
+    const Exponents e = exponents_of(m.pos[lane] != kNoKey, m.vs[lane]);
     if (lane == 0) m.e = e;
   };
-  int r_seen = -126;
+  int r_seen = -126, r_low = 127;
   auto finish = [&](int first, Meta& m) {                          // first: the ring's index of the four steps' first
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int e = uni(metas[first + i].e);
-      r_seen = e > r_seen ? e : r_seen;
+      const int top = uni(metas[first + i].e.top), low = uni(metas[first + i].e.low);
+      r_seen = top > r_seen ? top : r_seen;
+      r_low = low < r_low ? low : r_low;
     }
+    const bool wide = r_seen - r_low > kSpread;
     m.ks[lane] *= a.scale_log2;
-    m.vs[lane] = ldexpf(m.vs[lane], kPShift - r_seen);
-    if (lane == 0) m.r = r_seen;
+    const float vs = m.vs[lane];
+    m.vs[lane] = wide ? wide_mantissa(vs) : ldexpf(vs, kPShift - r_seen);
+    if (wide) m.ex[lane] = wide_exponent(vs);
+    if (lane == 0) m.r = wide ? kWide : r_seen;
   };
 
   // Bringing a step's bytes: of K a thread takes whole 16-byte pieces, of V four bytes of each of eight keys.
@@ -1029,12 +1095,18 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int c = 0; c < 16; ++c) o[i][c] *= by;
   };
 
+  auto shift_sums = [&](int by) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[i][c] = ldexpf(o[i][c], by);
+  };
+
   auto compute = [&](int t, int buf, const Meta& meta, int r, bool gone) {
+    const bool wide = r == kWide;
     if (r != r_exp) {
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[i][c] = ldexpf(o[i][c], r_exp - r);
+      if (wide) row_r[32 * wave + col] = r_exp;
+      shift_sums(wide ? 0 : r_exp - r);
       r_exp = r;
     }
     const bool edge = (t + 1) * kKeys > wave_all || gone;
@@ -1099,12 +1171,14 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-    if (__ballot(top > kSlack || (m_run == kMinusInf && top > kMinusInf))) {
+    const float counted = wide ? 0.f : 1.f;
+    if (wide || __ballot(top > kSlack || (m_run == kMinusInf && top > kMinusInf))) {
       top = fmaxf(top, __shfl_xor(top, 32));
       // a row moves if it has to or has no reference yet; its two lanes agree
       const bool move = top > kSlack || (m_run == kMinusInf && top > kMinusInf);
       const float by = move ? top : 0.f;
       const float grow = m_run == kMinusInf ? 0.f : exp2_fast(-by);
+      const float moved = m_run == kMinusInf ? __builtin_huge_valf() : by;
       if (move) m_run = from + by;
       l_run *= grow;
       scale_sums(grow);
@@ -1112,6 +1186,33 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] -= by;
+      if (wide) {                                    // l by itself; z then takes the scale's exponent along, relative to the row's r
+        float most = kMinusInf;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 ex = *reinterpret_cast<const f32x4*>(&meta.ex[32 * kb + 8 * i + 4 * half]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              l_run += exp2_fast(s[kb][4 * i + c]);
+              most = fmaxf(most, s[kb][4 * i + c] + ex[c]);
+            }
+          }
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const int was = row_r[32 * wave + col], r_now = row_exponent(was, moved, most);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        row_r[32 * wave + col] = r_now;
+        shift_sums(was - r_now);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 ex = *reinterpret_cast<const f32x4*>(&meta.ex[32 * kb + 8 * i + 4 * half]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[kb][4 * i + c] += ex[c] + (float)(kPShift - r_now);
+          }
+      }
     }
     f32x4 vs[2][4];
     auto read_vs = [&](int kb) {
@@ -1132,7 +1233,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e = exp2_fast(s[kb][i]);
-        l_run += e;
+        l_run = fmaf(e, counted, l_run);
         s[kb][i] = e * vs[kb][i / 4][i & 3];
       }
     };
@@ -1195,7 +1296,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
     lds_barrier();
     bring(metas[0]);
     wait_vmem<0>();
-    find_exponent(metas[wave]);
+    find_exponents(metas[wave]);
     lds_barrier();
     finish(0, metas[wave]);
     int gone = uni(metas[0].gone);
@@ -1209,7 +1310,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         copy_pages(t + 8 + wave);
       } else if ((i & 3) == 1) {
         wait_vmem<0>();                            // the scales, asked for a step ago
-        find_exponent(metas[ahead + wave]);
+        find_exponents(metas[ahead + wave]);
       } else if ((i & 3) == 3) {
         finish(ahead, metas[ahead + wave]);
       }
@@ -1233,6 +1334,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
 
   l_run += __shfl_xor(l_run, 32);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+  const int off = (r_exp == kWide ? row_r[32 * wave + col] : r_exp) - kPShift;       // what comes off the row's sums
   const Row me = my_row((int)opaque((uint32_t)col));
   const uint32_t tok = me.tok;
   const int head = me.head, r = me.r, by_half = (int)opaque((uint32_t)half);
@@ -1245,7 +1347,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
       for (int j = 0; j < 4; ++j) {
         float y[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, r_exp - kPShift);
+        for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, off);
         gstore<u32x2>(dst + 2 * (32 * i + 8 * j + 4 * by_half), u32x2{narrow<TYPE>(y[0], y[1]), narrow<TYPE>(y[2], y[3])});
       }
     if (a.lse && by_half == 0)
@@ -1260,7 +1362,7 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
         for (int j = 0; j < 4; ++j) {
           f32x4 y;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, r_exp - kPShift);
+          for (int c = 0; c < 4; ++c) y[c] = ldexpf(o[i][4 * j + c] * inv, off);
           gstore<f32x4>(dst + 4 * (32 * i + 8 * j + 4 * by_half), y);
         }
     }

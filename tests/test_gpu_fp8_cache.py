@@ -736,3 +736,126 @@ def test_refusals(bk, lib, cuda):
         for call in (lambda b: lib.bikv_fp8_attend(w.cache._h, 1, b, q.data_ptr(), 512, 128, 4, 1, 0.1, k.data_ptr(), 512, 128, None, q.data_ptr(), need, None),
                      lambda b: lib.bikv_fp8_append(w.cache._h, 1, b, k.data_ptr(), 256, 128, k.data_ptr(), 256, 128, None)):
             assert call(struct.pack("=7q2i", *f)) == _lib.EINVAL, (at, value)
+
+
+# ---- V scales far apart -------------------------------------------------------------------------
+def _weight_oracle(w, q, causal=True, layer=1):
+    """(out, lse, tolerance of out, tolerance of lse), float64, for pages of any V scale. A row's weights are p_j vs_j over the keys it sees, W the largest of them. A
+    weight is rounded to fp16's 11 bits (2^-12 of itself at most) or, far below W, to 2^-25 of W, and multiplies |byte| <= 448; what one bound or
+    the other leaves is doubled, for a weight is a product of rounded factors. z is summed in fp32 (dz), the n products too. The output's own
+    rounding is eps / 2, or half its type's smallest step."""
+    D, G, P = w.D, w.Hq // w.H, w.P
+    val = w.bytes[layer].view(FP8).double()
+    out = torch.zeros((w.rows, w.Hq, D), dtype=torch.float64)
+    lse = torch.full((w.rows, w.Hq), -math.inf, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    info = torch.finfo(w.t)
+    for b, (n, new) in enumerate(zip(w.lens, w.news)):
+        pages = w.table[b, :-(-n // P)]
+        r = slice(int(w.starts[b]), int(w.starts[b]) + new)
+        for h in range(w.Hq if n and new else 0):
+            k, v = (val[kv, pages][:, :, h // G].reshape(-1, D)[:n] for kv in (0, 1))
+            ks, vs = (w.scale[layer, kv][pages][:, h // G].double().repeat_interleave(P)[:n] for kv in (0, 1))
+            x = q[r, h].double() / math.sqrt(D)
+            z = (x @ k.t()) * ks
+            see = torch.arange(n)[None] < (n - new + 1 + torch.arange(new))[:, None] if causal else torch.ones(new, n, dtype=torch.bool)
+            dz = (D + 4) * 2.0 ** -24 * torch.where(see, (x.abs() @ k.abs().t()) * ks, torch.zeros_like(z)).amax(1)
+            z = torch.where(see, z, torch.full_like(z, -math.inf))
+            any_ = see.any(1)
+            lse[r, h] = torch.logsumexp(z, 1)
+            p = torch.where(see, torch.exp(z - torch.where(any_, lse[r, h], torch.zeros_like(lse[r, h]))[:, None]), torch.zeros_like(z))
+            weight = p * vs
+            out[r, h] = weight @ v
+            A, W = weight @ v.abs(), weight.amax(1, keepdim=True)
+            tol[r, h] = (info.eps / 2 * out[r, h].abs() + info.smallest_normal * info.eps / 2
+                         + A * (2.0 ** -11 + 2 * dz[:, None] + 2.0 ** -20 + (n + 8) * 2.0 ** -24) + n * 448 * W * 2.0 ** -24)
+            ltol[r, h] = dz + 2.0 ** -21 * (1 + torch.where(any_, lse[r, h].abs(), torch.zeros_like(dz))) + (n + 8) * 2.0 ** -24
+    return out, lse, tol, ltol
+
+
+def _check_weights(w, q, causal=True):
+    got = w.attend(q, causal=causal)
+    w.cache.check()
+    out, lse, tol, ltol = _weight_oracle(w, q, causal)
+    o, l = got[0].cpu().double(), got[1].cpu().double()
+    over = (o - out).abs() - tol
+    assert not (over > 0).any(), f"out is off by {float(((o - out).abs() / tol).max())} times what it may be"
+    none = lse == -math.inf
+    assert torch.equal(l == -math.inf, none) and ((l - lse).abs() <= ltol)[~none].all()
+
+
+FAR = [
+    # lens, new tokens, KV heads, q heads per KV head, head size, tokens of a page
+    ([200], [40], 2, 4, 128, 16),                                    # many rows
+    ([700, 300], [150, 130], 1, 2, 64, 16), ([300], [290], 1, 1, 128, 1), ([1500], [70], 1, 2, 128, 50),
+    ([200], [16], 2, 1, 128, 16),                                    # few: 16 rows
+    ([77, 200], [5, 3], 2, 4, 64, 8), ([600] + [40] * 9, [5] * 10, 1, 6, 128, 16),        # and 32
+    ([400, 90], [1, 1], 2, 8, 128, 16),                              # one token each: it sees every page
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("wide", [0, 9000])
+@pytest.mark.parametrize("apart", [5, 8, 9, 20, 26, 36, 150])
+@pytest.mark.parametrize("case", range(len(FAR)))
+def test_v_scales_of_later_pages_do_not_reach_earlier_rows(bk, cuda, case, apart, wide, dtype):
+    """The pages of a sequence's last tokens have V scales 2^apart larger than the ones before: the rows that see none of them keep all of their bits, and
+    the same holds the other way round for the rows that do."""
+    lens, news, H, G, D, P = FAR[case]
+    if dtype == "fp16" and apart > 36:
+        apart = 30                                                   # what lies farther apart is no fp16 number
+    w = World(bk, cuda, lens, news, P=P, H=H, D=D, Hq=G * H, dtype=dtype, seed=90 + case, wide=wide)
+    for b, (n, new) in enumerate(zip(lens, news)):
+        pages = w.table[b, :-(-n // P)]
+        late = pages[(n - -(-new // 2)) // P:]                       # the later half of the new tokens, and what shares their first page
+        w.scale[1, 1, pages] *= 2.0 ** (-70 if apart > 64 else 10 - apart)
+        w.scale[1, 1, late] *= 2.0 ** apart
+    w.push()
+    _check_weights(w, w.randn(w.Hq, 1.5))
+    _check_weights(w, w.randn(w.Hq, 1.5), causal=False)
+
+
+@pytest.mark.parametrize("dtype,apart", [("bf16", 36), ("fp16", 30)])
+@pytest.mark.parametrize("G", [1, 2])
+def test_v_scales_of_later_pages_in_the_same_step_of_a_wave(bk, cuda, G, dtype, apart):
+    """So many tiles that a head has one wave: it reads the last, far larger page together with pages that every row sees."""
+    lens = [90 + i % 9 for i in range(140)]
+    w = World(bk, cuda, lens, [16] * 140, H=8, D=64, Hq=8 * G, dtype=dtype, seed=105, wide=0)
+    for b, n in enumerate(lens):
+        w.scale[1, 1, w.table[b, :-(-n // 16)]] *= 2.0 ** (10 - apart)
+        w.scale[1, 1, w.table[b, (n - 1) // 16]] *= 2.0 ** apart
+    w.push()
+    _check_weights(w, w.randn(w.Hq, 1.5))
+
+
+@pytest.mark.parametrize("wide", [0, 9000])
+@pytest.mark.parametrize("case", range(len(FAR)))
+def test_v_scales_of_any_kind(bk, cuda, case, wide):
+    """Scales from 2^-90 to 2^70 page by page, zeros and the scale of an empty page among them; rows that hardly attend to the pages of large scale."""
+    lens, news, H, G, D, P = FAR[case]
+    w = World(bk, cuda, lens, news, P=P, H=H, D=D, Hq=G * H, seed=110 + case, wide=wide)
+    e = torch.randint(-90, 70, w.scale[1, 1].shape, generator=w.g).double()
+    w.scale[1, 1] = torch.exp2(e).float()
+    w.scale[1, 1, ::5] = 0.0
+    w.scale[1, 1, 3::5] = 2.0 ** -126
+    w.push()
+    _check_weights(w, w.randn(w.Hq, 1.5))
+    _check_weights(w, w.randn(w.Hq, 6.0), causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("wide", [0, 9000])
+@pytest.mark.parametrize("news,G", [([1], 4), ([16], 1), ([6], 5), ([150], 2)])
+def test_a_page_that_a_row_hardly_attends_to_takes_no_bits(bk, cuda, news, G, wide, dtype):
+    """Keys of the large V scale lie some 2^-60 below the others in the softmax: the others' values are what comes out."""
+    w = World(bk, cuda, [260], news, H=2, Hq=2 * G, dtype=dtype, seed=130, wide=wide)
+    w.bytes[1, 0] = 0x38                                             # every key is 1 in every place
+    w.scale[1, 0] = 2.0 ** -2
+    far = w.table[0, 2:9:3]
+    w.scale[1, 0, far] = 2.0 ** -7                                   # z = 16 sqrt(2) there ...
+    w.scale[1, 1] = 2.0 ** -20
+    w.scale[1, 1, far] = 2.0 ** (9 if dtype == "fp16" else 30)
+    w.push()
+    q = (1 + torch.rand((w.rows, w.Hq, 128), generator=w.g) * 0.1).to(w.t) * 16
+    _check_weights(w, q)
+    _check_weights(w, q, causal=False)
