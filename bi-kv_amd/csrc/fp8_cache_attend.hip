@@ -140,7 +140,6 @@ __device__ __forceinline__ int row_exponent(int r, float moved, float top) {
 // A tile that lies in one share is finished there; of the others each share leaves (O, m, l), and
 // fp8_join_few_kernel joins them.
 // ---------------------------------------------------------------------------------------------
-constexpr int kFewWaves = 8;               // of 256 registers: they fill a CU
 template <int D, int TYPE, int NT, int NK>
 struct Few {
   static constexpr int kM = 16 * NT;       // rows of a tile
@@ -193,9 +192,6 @@ __device__ __forceinline__ int64_t first_tile(const AttendArgs& a, int64_t b) {
   int64_t q = a.seq.q_starts[b];
   q = q < 0 ? 0 : q > a.seq.n_rows ? a.seq.n_rows : q;
   return q * a.group.d / M + b;
-}
-static int64_t tiles_in_all(bool one_each, int group, int64_t n_seqs, int64_t n_rows, int m) {
-  return one_each ? n_seqs * (((int64_t)group + m - 1) / m) : n_rows * group / m + n_seqs;
 }
 
 // The line's length (the host sees to it that it stays below 2^31).
@@ -875,8 +871,6 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // A tile's keys are cut into `slots` parts where the tiles alone would not fill the chip; the parts' results are
 // joined by fp8_join_many_kernel.
 // ---------------------------------------------------------------------------------------------
-constexpr int kManyRows = 128;
-constexpr int kManyKeys = 64;
 constexpr int kWide = 1 << 20;          // in r's place: the step is a wide one
 
 template <int TYPE>
@@ -1373,7 +1367,6 @@ __global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArg
   }
 }
 
-constexpr int kMostParts = 64;
 // Joins the parts of a tile's keys: D/4 threads a row, each with a share of the parts' (m, l) and four places over all parts, four
 // parts' places under way at a time.
 template <int D, int TYPE>
@@ -1440,67 +1433,6 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
 }
 
 // ---------------------------------------------------------------------------------------------
-AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, int64_t n_rows, int64_t max_len) {
-  AttendPlan p = {};
-  const int64_t all = n_rows * group;                      // rows of one KV head
-  const int64_t mean = (all + n_seqs - 1) / n_seqs;
-  // Up to 16 rows of a sequence on average: few rows (3 sequences of 32k, 8 KV heads, 16 rows: 58 us against 69 as many rows; 64 of
-  // 3000: 113 and 137). Up to 32: where the sequences are many enough for the shares (64 of 3000, 21 rows, 4 heads, 63 us against
-  // 119; 12 of 4500, 33 and 35; but 6 of 3000, 27 and 23; one of 20000, 43 and 30). More: many rows; a 64-row tile of the first
-  // kind took two to three times as long.
-  const int m = mean <= 16 ? 16 : 32, keys = m == 16 ? 64 : 32;
-  const int64_t tiles = tiles_in_all(one_each, group, n_seqs, n_rows, m);
-  if ((mean <= 16 || (mean <= 32 && n_seqs >= 8)) && tiles * ((max_len + keys - 1) / keys + 1 + 2 * kFewWaves) < (int64_t(1) << 31)) {   // the line's length fits 32 bits
-    p.form = m == 16 ? ATTEND_FEW_16 : ATTEND_FEW_32;
-    p.rows = m;
-    p.tiles = tiles;
-    const int waves = kFewWaves;
-    p.heads_per_group = heads < waves ? heads : waves;
-    if (max_len <= 1024) {
-      // A workgroup per tile, no second launch: 11.5 us against 16 for a sequence of 500 tokens, 15 against 16 at 1000; at 1500
-      // shares are ahead (18.7 against 17.1), and at 4000 by half (35 against 22). Where there are few tiles a head
-      // gets more waves, of more workgroups: 8 sequences of up to 2000 tokens take 22 us, 103 without; but
-      // no more workgroups than CUs, each of which holds one (42 short sequences 12.6 us, 19.4 in twice as many).
-      auto groups = [&](int32_t per) { return tiles * ((heads + per - 1) / per); };
-      while (p.heads_per_group > 1 && groups((p.heads_per_group + 1) / 2) <= 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
-      p.slots = 0;
-    } else {
-      // one workgroup for each of the 256 CUs, which is what one holds of this size
-      const int64_t slots = 256 / ((heads + p.heads_per_group - 1) / p.heads_per_group);
-      p.slots = (int32_t)(slots < 1 ? 1 : slots);
-    }
-    p.min_steps = waves / p.heads_per_group;
-    // 3 steps of each wave of a head: 64 sequences of 100 to 4000 tokens, 3 new each, 28 and 4 heads, take 51 us, 64 without and 59
-    // with one; 64 of 1k to 8k, 64 and 8 heads, 140, 148 and 144.
-    p.begin_cost = p.slots > 0 ? 3 * p.min_steps : 0;
-    p.part_rows = p.slots > 1 ? 2 * (int64_t)p.slots * heads * p.rows : 0;
-  } else {
-    p.form = ATTEND_MANY;
-    p.rows = kManyRows;
-    p.tiles = tiles_in_all(one_each, group, n_seqs, n_rows, kManyRows);
-    // Parts of a tile's keys. The chip holds 512 of these workgroups, two to a CU, so `n` of them take ceil(n / 512) rounds of their
-    // steps, and some two steps more to begin and to end (two again where empty workgroups, of tiles that sequences may have
-    // and these do not, take a place first); the parts' sums are written and read again, 115 of them in a step's time. 33 sequences of 40 to 64 rows over 4000 keys, 8 KV heads: 243 us in one part, 184 in three; 300 new
-    // tokens of each of 2 sequences of 3500, 4 KV heads: 52 us in 6 parts, 119 in one and 66 in 12. From 1024 tiles on the rounds
-    // even out by themselves. Parts have four steps at least, and their sums take 140 MB at most.
-    const int64_t tiles_likely = one_each ? p.tiles : all / kManyRows + n_seqs / 2, n = heads * (tiles_likely > n_seqs ? tiles_likely : n_seqs);
-    const int64_t steps = (max_len + kManyKeys - 1) / kManyKeys;
-    p.slots = 1;
-    if (n < 1024) {
-      int64_t least = -1;
-      for (int64_t parts = 1; parts <= kMostParts && (parts == 1 || (parts <= steps / 4 && p.tiles * heads * parts <= 2048)); ++parts) {
-        const int64_t cost = (n * parts + 511) / 512 * ((steps + parts - 1) / parts + 2) + (parts > 1 ? n * parts / 115 + 2 : 0) + (p.tiles * heads * parts > 512 ? 2 : 0);
-        if (least < 0 || cost < least) {
-          least = cost;
-          p.slots = (int32_t)parts;
-        }
-      }
-    }
-    p.part_rows = p.slots > 1 ? p.tiles * heads * p.slots * kManyRows : 0;
-  }
-  return p;
-}
-
 template <int D, int TYPE, int NT, int NK>
 static hipError_t launch_few(const AttendPlan& p, const AttendArgs& a, hipStream_t s) {
   const int64_t groups = (p.slots > 0 ? p.slots : p.tiles) * ((a.layer.heads + p.heads_per_group - 1) / p.heads_per_group);

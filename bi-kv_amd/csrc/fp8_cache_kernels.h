@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "host_logic/attend_plan.h"
 #include "host_logic/fp8_logic.h"
 
 namespace bikv {
@@ -76,19 +77,6 @@ struct AttendArgs {
   int64_t tiles;             // row tiles of the launch
   uint32_t* status;
 };
-enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_MANY = 2 };
-struct AttendPlan {
-  int form;
-  int rows;                  // rows of a tile
-  int32_t slots;
-  int32_t min_steps;
-  int32_t begin_cost;
-  int32_t heads_per_group;
-  int64_t tiles;
-  int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
-};
-// The form a call takes, from what the host knows of it alone. one_each: no row numbers, a sequence has one row.
-AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n_seqs, int64_t n_rows, int64_t max_len);
 hipError_t launch_fp8_attend(const AttendPlan& plan, int head_dim, int type, const AttendArgs& a, hipStream_t stream);
 
 }  // namespace bikv

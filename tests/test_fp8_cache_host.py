@@ -74,6 +74,36 @@ int main() {
     assert out == ["0"]
 
 
+def test_the_line_of_few_rows_work_stays_below_2_31(tmp_path):
+    """Every tile's key steps and what beginning it costs, for as many tiles as a call may have: signed 32-bit numbers count them."""
+    out = _run_c(tmp_path, r"""
+#include <stdio.h>
+#include <initializer_list>
+#include "host_logic/attend_plan.h"
+int main() {
+  long bad = 0, few = 0, n = 0, close = 0;
+  for (int heads : {1, 2, 3, 5, 8, 9, 1024})
+    for (int group : {1, 4, 7, 16, 32})
+      for (int one_each : {0, 1})
+        for (int64_t seqs : {int64_t(1), int64_t(9), int64_t(1000), int64_t(1) << 20, (int64_t(1) << 24) - 1})
+          for (int64_t rows_each : {1, 2, 4, 8, 16, 31})
+            for (int64_t len = 0; len <= (int64_t(1) << 30); len = len < 4096 ? len + 32 : len * 2 + 1) {
+              const int64_t rows = one_each ? seqs : seqs * rows_each;
+              if (rows >= (int64_t(1) << 30)) continue;
+              const bikv::AttendPlan p = bikv::plan_fp8_attend(heads, group, one_each, seqs, rows, len);
+              ++n;
+              if (p.form == bikv::ATTEND_MANY) continue;
+              const int64_t line = p.tiles * (bikv::steps_of_keys(len, p.form == bikv::ATTEND_FEW_16 ? 64 : 32) + p.begin_cost);
+              ++few;
+              bad += line >= (int64_t(1) << 31);
+              close += line > (int64_t(1) << 31) / 10 * 9;
+            }
+  printf("%ld %ld %ld %ld\n", bad, few, n, close);
+}
+""")
+    assert out[0] == "0" and int(out[1]) > 10000 and int(out[3]) > 5
+
+
 def test_structs_agree_with_the_header(lib, tmp_path):
     from bikv_pagecopy import _lib, fp8_cache
     fields = [n for n, _ in _lib.FP8CacheDesc._fields_]
