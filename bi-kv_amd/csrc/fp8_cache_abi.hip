@@ -130,8 +130,8 @@ extern "C" int bikv_fp8_append(const bikv_fp8_cache* c, int32_t layer, const bik
   a.k_head = k_head_stride;
   a.v_row = v_row_stride;
   a.v_head = v_head_stride;
-  a.units = b->q_starts ? b->n_rows / c->page_tokens + 2 * b->n_seqs : b->n_seqs;
-  if (a.units * 2 * c->heads >= (int64_t(1) << 31)) return fail(BIKV_ERANGE, "too many pages times heads for one call");
+  a.units = append_units(!b->q_starts, b->n_seqs, b->n_rows, c->page_tokens);
+  if (!launch_fits(append_groups(a.units, c->heads), kAppendThreads)) return fail(BIKV_ERANGE, "too many pages times heads for one call");
   rc = device_status(c->device, ST_BANK_SHARED, &a.status);
   if (rc) return rc;
   BIKV_DEVICE(c->device);
@@ -152,7 +152,7 @@ static int plan_call(const bikv_fp8_cache* c, const bikv_seq_batch* b, int32_t q
   *plan = AttendPlan();
   if (b->n_seqs == 0 || b->n_rows == 0) return BIKV_OK;
   *plan = plan_fp8_attend(c->heads, q_heads / c->heads, !b->q_starts, b->n_seqs, b->n_rows, b->max_pages * c->page_tokens);
-  if (plan->tiles * c->heads * (plan->form == ATTEND_MANY ? plan->slots * 32 : 1) >= (int64_t(1) << 31))
+  if (!launch_fits(plan->groups, plan->threads))       // the joins' launches are smaller
     return fail(BIKV_ERANGE, "too many rows times heads for one call");
   return BIKV_OK;
 }

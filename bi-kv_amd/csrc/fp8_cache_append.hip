@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t pack4_scaled(uint32_t ab, uint32_t cd, float
 }
 
 template <int D, int TYPE>
-__global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(kAppendThreads) void fp8_append_kernel(const AppendArgs a) {
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRows = 64 / kLanesPerRow;    // rows a wave reads with one instruction
   constexpr int kVecs = 8, kOld = 4;
@@ -240,8 +240,7 @@ __global__ __launch_bounds__(256) void fp8_append_kernel(const AppendArgs a) {
 }
 
 hipError_t launch_fp8_append(int head_dim, int type, const AppendArgs& a, hipStream_t stream) {
-  const int64_t waves = a.units * 2 * a.layer.heads;
-  const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
+  const dim3 grid((uint32_t)append_groups(a.units, a.layer.heads)), block(kAppendThreads);
   if (head_dim == 128) {
     if (type == 0) hipLaunchKernelGGL((fp8_append_kernel<128, 0>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((fp8_append_kernel<128, 1>), grid, block, 0, stream, a);

@@ -882,7 +882,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 template <int D, int TYPE>
-__global__ __launch_bounds__(256, 2) void fp8_attend_many_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(kManyThreads, 2) void fp8_attend_many_kernel(const AttendArgs a) {
   constexpr int kKeys = kManyKeys;
   constexpr int kChunks = D / 8;                  // 16-byte pieces of a K row in LDS
   constexpr int kLoads = D / 64;                  // 16-byte pieces of K a thread brings per step
@@ -1435,8 +1435,8 @@ __global__ __launch_bounds__(256) void fp8_join_many_kernel(const AttendArgs a) 
 // ---------------------------------------------------------------------------------------------
 template <int D, int TYPE, int NT, int NK>
 static hipError_t launch_few(const AttendPlan& p, const AttendArgs& a, hipStream_t s) {
-  const int64_t groups = (p.slots > 0 ? p.slots : p.tiles) * ((a.layer.heads + p.heads_per_group - 1) / p.heads_per_group);
-  hipLaunchKernelGGL((fp8_attend_few_kernel<D, TYPE, NT, NK>), dim3((uint32_t)groups), dim3(64 * Few<D, TYPE, NT, NK>::kWaves), 0, s, a);
+  static_assert(Few<D, TYPE, NT, NK>::kWaves == kFewWaves, "the plan's workgroup");
+  hipLaunchKernelGGL((fp8_attend_few_kernel<D, TYPE, NT, NK>), dim3((uint32_t)p.groups), dim3(p.threads), 0, s, a);
   if (p.slots > 1) hipLaunchKernelGGL((fp8_join_few_kernel<D, TYPE, 16 * NT>), dim3((uint32_t)(p.slots * a.layer.heads), 4 * NT), dim3(256), 0, s, a);
   return hipGetLastError();
 }
@@ -1448,7 +1448,7 @@ static hipError_t launch_form(const AttendPlan& p, const AttendArgs& a, hipStrea
     case ATTEND_FEW_32: return launch_few<D, TYPE, 2, 2>(p, a, s);
     default: break;
   }
-  hipLaunchKernelGGL((fp8_attend_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * p.slots)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((fp8_attend_many_kernel<D, TYPE>), dim3((uint32_t)p.groups), dim3(p.threads), 0, s, a);
   if (p.slots > 1)
     hipLaunchKernelGGL((fp8_join_many_kernel<D, TYPE>), dim3((uint32_t)(p.tiles * a.layer.heads * (kManyRows * D / 1024))), dim3(256), 0, s, a);
   return hipGetLastError();

@@ -9,6 +9,7 @@ enum : int { ATTEND_FEW_16 = 0, ATTEND_FEW_32 = 1, ATTEND_MANY = 2 };
 constexpr int kFewWaves = 8;             // waves of a few rows' workgroup, of 256 registers: they fill a CU
 constexpr int kManyRows = 128;           // rows of a many rows' tile
 constexpr int kManyKeys = 64;            // and its keys a step
+constexpr int kManyThreads = 256;
 constexpr int kMostParts = 64;           // a tile's keys are cut into no more
 
 struct AttendPlan {
@@ -20,6 +21,8 @@ struct AttendPlan {
   int32_t heads_per_group;
   int64_t tiles;
   int64_t part_rows;         // rows of partial results the call may need (x head_dim floats + 2 floats)
+  int64_t groups;            // workgroups of the launch that reads the cache, and their threads
+  int threads;
 };
 
 // Row tiles of `m` rows: with one token each the sequences have as many tiles each; else every sequence may leave one unfilled.
@@ -64,6 +67,8 @@ inline AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n
     p.min_steps = waves / p.heads_per_group;
     p.begin_cost = p.slots > 0 ? begin_cost : 0;             // the heads of a workgroup are as they were, then
     p.part_rows = p.slots > 1 ? 2 * (int64_t)p.slots * heads * p.rows : 0;
+    p.groups = (p.slots > 0 ? p.slots : p.tiles) * ((heads + p.heads_per_group - 1) / p.heads_per_group);
+    p.threads = 64 * kFewWaves;
   } else {
     p.form = ATTEND_MANY;
     p.rows = kManyRows;
@@ -87,6 +92,8 @@ inline AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n
       }
     }
     p.part_rows = p.slots > 1 ? p.tiles * heads * p.slots * kManyRows : 0;
+    p.groups = p.tiles * heads * p.slots;
+    p.threads = kManyThreads;
   }
   return p;
 }

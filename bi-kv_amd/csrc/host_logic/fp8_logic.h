@@ -26,6 +26,15 @@ inline FastDiv fast_div(uint32_t d) {
 }
 BIKV_HD uint32_t divide(uint32_t n, const FastDiv& f) { return (uint32_t)((n * f.mul) >> f.shift); }
 
+// Threads of a launch are numbered with 32 bits.
+inline bool launch_fits(int64_t groups, int64_t threads_each) { return groups < (int64_t(1) << 32) / threads_each; }
+
+// append: a wave for each page slot, K or V, and head, four to a workgroup. With row numbers there are as many slots as n_rows tokens of n_seqs
+// sequences can touch pages.
+constexpr int kAppendThreads = 256;
+inline int64_t append_units(bool one_each, int64_t n_seqs, int64_t n_rows, int page_tokens) { return one_each ? n_seqs : n_rows / page_tokens + 2 * n_seqs; }
+inline int64_t append_groups(int64_t units, int heads) { return (units * 2 * heads + 3) / 4; }
+
 // `total` steps of work in at most `slots` equal shares of at least `min_steps`: slot s has [begin, end), step x
 // lies in share x / per.
 struct Share {

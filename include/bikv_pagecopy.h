@@ -481,7 +481,9 @@ int bikv_nhd_store_token_major(const bikv_nhd* pool, void* tm, int64_t tm_bytes,
  * tensors, for append more rows than tokens) is skipped as a whole and raises BIKV_ST_SRC_RANGE; a page id outside the pool
  * raises BIKV_ST_PAGE_ID and its tokens are left out. Asynchronous on `stream`, no allocation, graph-capturable.
  * Row and head strides are in elements, multiples of 8; addresses are 16-byte aligned; a head's values are contiguous.
- * max_pages * page_tokens is at most 2^30, n_rows below 2^30, n_seqs below 2^24 (BIKV_ERANGE).
+ * max_pages * page_tokens is at most 2^30, n_rows below 2^30, n_seqs below 2^24, and a call's work fits one launch of 2^32 threads: for
+ * append up to 2^25 pages (n_rows / page_tokens + 2 n_seqs with row numbers) times kv_heads, for attend some 2^31 n_rows times q_heads or, of single
+ * tokens over short tables, 2^23 sequences times eighths of kv_heads (BIKV_ERANGE).
  * ------------------------------------------------------------------------------------------ */
 typedef struct bikv_fp8_cache bikv_fp8_cache; /* opaque; host memory only */
 

@@ -104,6 +104,32 @@ int main() {
     assert out[0] == "0" and int(out[1]) > 10000 and int(out[3]) > 5
 
 
+def test_launches_of_more_threads_than_a_launch_numbers_do_not_fit(tmp_path):
+    out = _run_c(tmp_path, r"""
+#include <stdio.h>
+#include "host_logic/attend_plan.h"
+#include "host_logic/fp8_logic.h"
+using namespace bikv;
+static int attend(int heads, int group, bool one_each, int64_t seqs, int64_t rows, int64_t len) {
+  const AttendPlan p = plan_fp8_attend(heads, group, one_each, seqs, rows, len);
+  const bool fits = launch_fits(p.groups, p.threads);
+  return fits == (p.groups * p.threads < (int64_t(1) << 32)) ? fits : -1;
+}
+static int append(int heads, bool one_each, int64_t seqs, int64_t rows, int page) {
+  const int64_t groups = append_groups(append_units(one_each, seqs, rows, page), heads);
+  return launch_fits(groups, kAppendThreads) == (groups * kAppendThreads < (int64_t(1) << 32)) ? launch_fits(groups, kAppendThreads) : -1;
+}
+int main() {
+  printf("%d%d%d%d ", launch_fits((int64_t(1) << 24) - 1, 256), launch_fits(int64_t(1) << 24, 256), launch_fits((int64_t(1) << 23) - 1, 512), launch_fits(int64_t(1) << 23, 512));
+  printf("%d%d%d%d ", append(64, false, 1, 600000, 1), append(64, false, 1, 500000, 1), append(8, true, 4000000, 4000000, 16), append(8, true, 1 << 23, 1 << 23, 16));
+  printf("%d%d%d%d ", attend(9, 1, true, 5000000, 5000000, 1000), attend(9, 1, true, 4000000, 4000000, 1000), attend(9, 1, true, 5000000, 5000000, 2000), attend(8, 1, false, 8, 1 << 29, 4096));
+  printf("%d\n", attend(1024, 4, false, 1 << 20, 1 << 24, 64));
+}
+""")
+    # the last five: 5 and 4 million workgroup pairs of 512 threads; shares, which are few whatever the call; 2^22 tiles of 8 heads; 2^20 of 1024
+    assert out == ["1010", "0110", "0110", "0"]
+
+
 def test_structs_agree_with_the_header(lib, tmp_path):
     from bikv_pagecopy import _lib, fp8_cache
     fields = [n for n, _ in _lib.FP8CacheDesc._fields_]

@@ -859,3 +859,19 @@ def test_a_page_that_a_row_hardly_attends_to_takes_no_bits(bk, cuda, news, G, wi
     q = (1 + torch.rand((w.rows, w.Hq, 128), generator=w.g) * 0.1).to(w.t) * 16
     _check_weights(w, q)
     _check_weights(w, q, causal=False)
+
+
+def test_calls_of_more_work_than_a_launch_has_threads_for_are_refused(bk, lib, cuda):
+    """As what they are, and before anything is launched: the sizes are numbers here, no memory stands behind them."""
+    from bikv_pagecopy import _lib
+    cache = bk.FP8KVCache(torch.zeros(1, 2, 4, 1, 64, 64, dtype=torch.uint8, device=cuda), torch.ones(1, 2, 4, 64, device=cuda))
+    x = torch.zeros(64, 64, 64, dtype=torch.bfloat16, device=cuda)
+    table, lens, starts = (torch.zeros(n, dtype=torch.int64, device=cuda) for n in (4, 4, 5))
+    at = lambda seqs, rows, pages, starts: struct.pack("=7q2i", table.data_ptr(), pages, pages, lens.data_ptr(), starts, seqs, rows, 0, 0)
+    for batch in (at(1, 600000, 4, starts.data_ptr()), at(1 << 20, 1 << 20, 4, 0)):
+        assert lib.bikv_fp8_append(cache._h, 0, batch, x.data_ptr(), 4096, 64, x.data_ptr(), 4096, 64, None) == _lib.ERANGE
+        assert "too many" in _lib.last_error()
+    for batch in (at(5000000, 5000000, 4, 0), at(1 << 20, 1 << 26, 4, starts.data_ptr())):
+        assert lib.bikv_fp8_attend_workspace(cache._h, batch, 64) == _lib.ERANGE
+        assert lib.bikv_fp8_attend(cache._h, 0, batch, x.data_ptr(), 4096, 64, 64, 1, 0.1, x.data_ptr(), 4096, 64, None, None, 0, None) == _lib.ERANGE
+    cache.check()
