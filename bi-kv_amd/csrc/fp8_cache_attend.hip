@@ -152,12 +152,15 @@ struct Few {
 
 // Global memory straight into LDS: lane i's 16 (4) bytes land at `lds` + 16 i (4 i). Written out so that the kernel
 // itself says which copies it waits for: the compiler would wait for all of them before any read of LDS.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"      // m0 is a reserved register: named all the same, for the compiler keeps values in it
 __device__ __forceinline__ void copy16_to_lds(uint64_t src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
 }
 __device__ __forceinline__ void copy4_to_lds(uint64_t src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Waits until at most N of the wave's newest vector memory accesses are under way.
 template <int N>
 __device__ __forceinline__ void wait_vmem() {

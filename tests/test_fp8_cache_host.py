@@ -1,6 +1,7 @@
 """The 8-bit cache and the page copies without a GPU: the kernels' integer arithmetic, the C structs, what is refused."""
 import ctypes as C
 import os
+import re
 import subprocess
 import types
 
@@ -128,6 +129,21 @@ int main() {
 """)
     # the last five: 5 and 4 million workgroup pairs of 512 threads; shares, which are few whatever the call; 2^22 tiles of 8 heads; 2^20 of 1024
     assert out == ["1010", "0110", "0110", "0"]
+
+
+def test_assembly_that_writes_m0_says_so():
+    """The compiler keeps values of its own in m0."""
+    csrc = os.path.join(ROOT, "bi-kv_amd", "csrc")
+    found = 0
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith((".hip", ".h")):
+            with open(os.path.join(csrc, name)) as f:
+                text = f.read()
+            for stmt in re.findall(r"\basm\b[^;]*;", text):
+                if re.search(r"\bs_mov_b32 m0\b", stmt):
+                    found += 1
+                    assert '"m0")' in stmt, (name, stmt)
+    assert found >= 2
 
 
 def test_structs_agree_with_the_header(lib, tmp_path):
