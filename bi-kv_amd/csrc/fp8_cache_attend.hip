@@ -22,6 +22,8 @@
 // does not see, or hardly attends to, takes no bits from the pages it does. They cost few rows 3 to 8 %, many rows a third.
 #include "fp8_cache_device.h"
 
+#include <cstddef>
+
 namespace bikv {
 
 constexpr float kMinusInf = -__builtin_huge_valf();
@@ -245,6 +247,7 @@ __global__ __launch_bounds__((64 * Few<D, TYPE, NT, NK>::kWaves), 2) void fp8_at
     int nan_at[D];                         // by place: the first key with a NaN in V that not every row sees
     int r[kM];                             // wide steps: the rows' r
   };
+  static_assert(offsetof(Meta, ks) % 16 == 0 && offsetof(Meta, vs) % 16 == 0 && offsetof(Meta, ex) % 16 == 0 && sizeof(Meta) % 16 == 0, "");
   __shared__ Meta metas[kWaves];
   __shared__ float sums[kWaves][2][kM];    // the waves' m and l
   const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63;
@@ -890,7 +893,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void fp8_attend_many_kernel(const 
   constexpr int kChunks = D / 8;                  // 16-byte pieces of a K row in LDS
   constexpr int kLoads = D / 64;                  // 16-byte pieces of K a thread brings per step
   constexpr int kRowThreads = D / 4;              // threads that bring one row of V, four bytes each
-  struct Meta {
+  struct alignas(16) Meta {                       // four floats are read at a time
     uint64_t off[kKeys];
     float ks[kKeys], vs[kKeys];                   // as they are in the cache; then times the softmax's scale and log2(e), and times 2^(kPShift - r)
     float ex[kKeys];                              // wide steps: the exponents of the V scales, whose mantissas are in vs then
@@ -898,6 +901,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void fp8_attend_many_kernel(const 
     int gone, r;                                  // some key is nobody's; the largest exponent of V's scales up to here, or kWide
     Exponents e;                                  // of V's scales here
   };
+  static_assert(offsetof(Meta, ks) % 16 == 0 && offsetof(Meta, vs) % 16 == 0 && offsetof(Meta, ex) % 16 == 0 && sizeof(Meta) % 16 == 0, "");
   __shared__ uint32_t pids_in[4][2][kKeys];       // page ids of the keys to be looked up next, low and high words
   __shared__ int nan_at[D];                       // by place: the first key with a NaN in V that not every row sees
   __shared__ int spoilt;

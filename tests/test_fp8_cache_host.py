@@ -146,6 +146,16 @@ def test_assembly_that_writes_m0_says_so():
     assert found >= 2
 
 
+def test_lds_that_is_read_four_floats_at_a_time_is_aligned_for_it():
+    """A struct without a 16-byte member is where the compiler likes to put it, unless it says what it needs."""
+    with open(os.path.join(ROOT, "bi-kv_amd", "csrc", "fp8_cache_attend.hip")) as f:
+        structs = re.findall(r"struct (alignas\(16\) )?Meta \{(.*?)\n  \};(.*?)\n  __shared__", f.read(), re.S)
+    assert len(structs) == 2
+    for aligned, members, after in structs:
+        assert aligned or "u32x4" in members
+        assert all(f"offsetof(Meta, {m}) % 16 == 0" in after for m in ("ks", "vs", "ex"))
+
+
 def test_structs_agree_with_the_header(lib, tmp_path):
     from bikv_pagecopy import _lib, fp8_cache
     fields = [n for n, _ in _lib.FP8CacheDesc._fields_]
