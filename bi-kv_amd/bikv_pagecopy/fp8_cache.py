@@ -23,6 +23,7 @@ import struct
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .pool import PagedKVPool, current_raw_stream
@@ -34,6 +35,11 @@ _TYPES = {torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_FP16}
 def _end(t: torch.Tensor) -> int:
     """Address behind the last element of a tensor that has one."""
     return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _has_tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None
 
 
 class FP8KVCache:
@@ -107,6 +113,8 @@ class FP8KVCache:
             raise RuntimeError(f"{name}: the values of a head must be contiguous")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, and the cache's calls record none: detach it or call under torch.no_grad()")
+        if _has_tangent(t):
+            raise RuntimeError(f"{name} carries a forward-mode gradient, and the cache's calls record none: pass its primal")
         return stride
 
     def _batch(self, rows, page_table, kv_lens, q_starts):

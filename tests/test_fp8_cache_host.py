@@ -236,6 +236,23 @@ def test_rows_that_the_kernels_cannot_read_are_refused(lib):
         c._rows("q", wants, None)
 
 
+def test_tensors_with_a_forward_mode_gradient_are_refused(lib):
+    """A tangent would be lost without a word, under no_grad too, which turns off the other mode only."""
+    import torch.autograd.forward_ad as fa
+    c = _bare()
+    x = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with fa.dual_level():
+        dual = fa.make_dual(x, torch.ones_like(x))
+        for t in (dual, dual[1:], dual[:, :1]):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                c._rows("q", t, None)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                c._rows("q", t, None)
+        c._rows("q", x, None)
+        c._rows("q", fa.unpack_dual(dual).primal, None)
+    c._rows("q", dual, None)                                 # the level is gone, and the tangent with it
+
+
 def test_sequence_arrays_that_are_not_what_a_call_takes_are_refused(lib):
     c = _bare()
     k = torch.zeros(3, 2, 128, dtype=torch.bfloat16)

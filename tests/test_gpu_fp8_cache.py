@@ -875,3 +875,18 @@ def test_calls_of_more_work_than_a_launch_has_threads_for_are_refused(bk, lib, c
         assert lib.bikv_fp8_attend_workspace(cache._h, batch, 64) == _lib.ERANGE
         assert lib.bikv_fp8_attend(cache._h, 0, batch, x.data_ptr(), 4096, 64, 64, 1, 0.1, x.data_ptr(), 4096, 64, None, None, 0, None) == _lib.ERANGE
     cache.check()
+
+
+def test_tensors_with_a_forward_mode_gradient_are_refused(bk, cuda):
+    import torch.autograd.forward_ad as fa
+    w = World(bk, cuda, [40, 20], [1, 1], H=2, Hq=4, seed=140, ragged=False)
+    k, q = w.randn(2).to(cuda), w.randn(4).to(cuda)
+    with fa.dual_level():
+        dual = lambda x: fa.make_dual(x, torch.ones_like(x))
+        for bad in (lambda: w.cache.attend(1, dual(q), w.table_d, w.lens_d), lambda: w.cache.append(1, dual(k), k, w.table_d, w.lens_d),
+                    lambda: w.cache.append(1, k, dual(k), w.table_d, w.lens_d), lambda: w.cache.attend(1, q, w.table_d, w.lens_d, out=dual(q.clone()))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                bad()
+        w.cache.attend(1, q, w.table_d, w.lens_d)
+    w.cache.check()
+    assert torch.equal(w.payload_d.cpu().view(torch.uint8), w.bytes)
