@@ -53,6 +53,7 @@ class FP8KVCache:
             raise RuntimeError("scale must be [layers, 2, pages, kv_heads]")
         PagedKVPool._check_plane(payload)
         PagedKVPool._check_plane(scale)
+        self._refuse_gradients((payload, scale))
         self._open([payload[l, k] for l in range(payload.shape[0]) for k in (0, 1)],
                    [scale[l, k] for l in range(payload.shape[0]) for k in (0, 1)])
 
@@ -65,6 +66,7 @@ class FP8KVCache:
 
     def _open(self, planes, scales):
         self._h = None
+        self._refuse_gradients(planes + scales)
         p0 = planes[0] if planes else None
         if p0 is None or len(planes) % 2 or len(scales) != len(planes):
             raise RuntimeError("a cache has a K and a V plane per layer, and a scale plane to each")
@@ -96,6 +98,11 @@ class FP8KVCache:
         self._default_scale = 1.0 / math.sqrt(self.head_dim)
         self._workspace = {}
         self.pool = PagedKVPool.from_planes(planes, scales)      # keeps the tensors alive, too
+
+    @staticmethod
+    def _refuse_gradients(tensors):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or any(_has_tangent(t) for t in tensors):
+            raise RuntimeError("a cache's payload and scale are written in place and record no gradient: detach them or make the cache under torch.no_grad()")
 
     # ---- arguments ----------------------------------------------------------------------------
     # A step calls these once per layer, so the checks are few expressions and what is wrong is found out afterwards.

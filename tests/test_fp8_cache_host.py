@@ -253,6 +253,21 @@ def test_tensors_with_a_forward_mode_gradient_are_refused(lib):
     c._rows("q", dual, None)                                 # the level is gone, and the tangent with it
 
 
+def test_a_cache_over_tensors_that_want_a_gradient_is_refused(lib):
+    """Attention over a scale that is learnt would leave it without a gradient."""
+    import torch.autograd.forward_ad as fa
+    from bikv_pagecopy import FP8KVCache
+    scale = torch.ones(3, 2)
+    for wants in ([scale, scale.clone().requires_grad_()], [torch.nn.Parameter(scale)]):
+        with pytest.raises(RuntimeError, match="gradient"):
+            FP8KVCache._refuse_gradients(wants)
+        with torch.no_grad():
+            FP8KVCache._refuse_gradients(wants)
+    FP8KVCache._refuse_gradients([scale])
+    with fa.dual_level(), pytest.raises(RuntimeError, match="gradient"):
+        FP8KVCache._refuse_gradients([fa.make_dual(scale, scale)])
+
+
 def test_sequence_arrays_that_are_not_what_a_call_takes_are_refused(lib):
     c = _bare()
     k = torch.zeros(3, 2, 128, dtype=torch.bfloat16)

@@ -890,3 +890,15 @@ def test_tensors_with_a_forward_mode_gradient_are_refused(bk, cuda):
         w.cache.attend(1, q, w.table_d, w.lens_d)
     w.cache.check()
     assert torch.equal(w.payload_d.cpu().view(torch.uint8), w.bytes)
+
+
+def test_a_cache_over_tensors_that_want_a_gradient_is_refused(bk, cuda):
+    w = World(bk, cuda, [40], [1], H=2, Hq=4, seed=141, ragged=False)
+    learnt = w.scale_d.clone().requires_grad_()
+    planes = [w.payload_d[l, kv] for l in range(2) for kv in (0, 1)]
+    scales = [w.scale_d[l, kv] for l in range(2) for kv in (0, 1)]
+    for make in (lambda: bk.FP8KVCache(w.payload_d, learnt), lambda: bk.FP8KVCache.from_planes(planes, scales[:3] + [scales[3].clone().requires_grad_()])):
+        with pytest.raises(RuntimeError, match="gradient"):
+            make()
+        with torch.no_grad():
+            make().close()
