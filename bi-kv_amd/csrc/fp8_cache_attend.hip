@@ -1146,13 +1146,6 @@ __global__ __launch_bounds__(kManyThreads, 2) void fp8_attend_many_kernel(const 
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) s[1] = mfma32<TYPE>(kf[j], q[j], s[1]);
     take_z(0);
-    if constexpr (TYPE == 1) {
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (j >= D / 32) __builtin_amdgcn_sched_group_barrier(0x2, 512 / D, 0);
-      }
-    }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (D != 64) read_ks(1);
     __builtin_amdgcn_sched_barrier(0);
@@ -1268,16 +1261,6 @@ __global__ __launch_bounds__(kManyThreads, 2) void fp8_attend_many_kernel(const 
         read_v(1, s2, dt);
       }
     weights(1);
-    // with fp16's twice as many products the order is given: a 4096-token prompt takes 276 us, 297 in the compiler's own
-    // order; bf16's is as fast in the compiler's
-    if constexpr (TYPE == 1) {
-#pragma unroll
-      for (int i = 0; i < 2 * (D / 32); ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 768 / D, 0);
-      }
-    }
     if (edge) blank(1);
     pack(1);
     __builtin_amdgcn_sched_barrier(0);
