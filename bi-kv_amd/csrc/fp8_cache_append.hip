@@ -21,7 +21,8 @@
 // at a time by the conversion that takes a power of two along; only a page with a NaN or an infinity, or an old scale that is no
 // power of two, goes value by value (with that for all, 29 us where it is 21 now). No LDS, no barrier, no atomics.
 // Measured: 16k tokens of 16 prompts, 8 heads of 128: 98 MB in 21 us, 4.7 TB/s; 9 chunks of up to 299 tokens
-// in pages of 50: 7 us; one token to each of 8 sequences: 4 us, a launch and the lookups.
+// in pages of 50: 7.6 us; one token to each of 8 sequences: 4.2 us, a launch and the lookups. Where every touched page outgrows its scale,
+// and its older rows are rounded again, these take 21, 7.9 and 5.8 us.
 #include "fp8_cache_device.h"
 
 namespace bikv {

@@ -30,8 +30,8 @@ constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr int kNoKey = 0x7fffffff;      // position of a key that no row sees
 constexpr int kPShift = 8;              // p is scaled by 2^8 in fp16: p down to 2^-22 stays normal
 // z is taken against a row's last reference m, which moves only when some z exceeds it by more than this: p may be up to 2^4, p
-// 2^kPShift vs 2^-r < 2^(4 + 8 + 1) is in fp16's range, and most steps rescale nothing and reduce nothing across lanes. With 0,
-// chunks of 900 behind 8192 tokens take 704 us where they take 682 with 4.
+// 2^kPShift vs 2^-r < 2^(4 + 8 + 1) is in fp16's range, and most steps rescale nothing and reduce nothing across lanes. With 0
+// 6 chunks of up to 900 tokens behind up to 8192 take 789 us where they take 777 with 4.
 constexpr float kSlack = 4.f;
 constexpr int kSpread = 8;
 constexpr int kLeastR = -400;           // below any exponent that is left over in a sum
@@ -122,15 +122,17 @@ __device__ __forceinline__ int row_exponent(int r, float moved, float top) {
 // heads; where there are more waves than heads, several waves share a head and take its steps in turn.
 //
 // Measured, with fp8_join_few_kernel: 64 sequences of 1024 to 8192 tokens, 64 query and 8 KV heads of 128, bf16, one new token
-// each: 612 MB in 118 + 7 us, 5.2 TB/s while the first kernel runs; 3 of 32k, 32 heads: 186 MB in 37 + 8 us; 24 of up to 5000
-// with up to 5 new tokens, 28 and 4 heads: 69 MB in 30 + 6 us, some 1.4 us of instructions to a step of a 32-row tile, whose
-// loads are no longer what it waits for (twice the buffers changed nothing); one of 777, 12 and 2 heads: 12.5 us, where what counts
-// is the chain of lookups (lengths, page ids, scales and rows) and how long code and data take to arrive.
+// each: 612 MB in 118 + 7 us, 5.2 TB/s while the first kernel runs; 3 of 32k, 32 heads: 186 MB in 37 + 8 us. 24 of up to 5000
+// with up to 5 new tokens, 28 and 4 heads: 69 MB in 30 + 6 us; by time stamps its workgroups take 23.5 us on average and 30 at most: 2 to find
+// their share, 2 until a tile's first rows are there, 11 for 5 steps (2.2 us each; twice the buffers changed nothing), 6 until the waves
+// of a head have joined their sums, the waiting for the slowest of them included. One of 777, 12 and 2 heads: 13 us; 1.8 to find the tile, 2 until the
+// first rows are there, 4 for two steps, 4 to join eight waves; the rest is the launch.
 //
 // Bound by memory: every byte of K and V is read once per row tile. Each wave copies its own steps' rows into its own part
 // of LDS (global_load_lds, 16 bytes a lane, whole rows) and never waits for another wave while it goes: scales and the next
 // page ids first, then K, then V, each refilled for the next step as soon as it has been read, with the waits
-// counted by hand. The heads of a page stand side by side in memory, so the waves of a workgroup together read whole
+// counted by hand. Eight waves of 256 registers fill a CU; for D = 128 that is not quite enough: 32-row tiles spill 19 (bf16) or 26 (fp16) of
+// them, 16-row tiles of fp16 3, where a tile begins and ends. The heads of a page stand side by side in memory, so the waves of a workgroup together read whole
 // pages: copies alone run at 6.2 TB/s this way and at 5.2 TB/s with every head in a workgroup of its own. From LDS a lane takes its
 // operands' bytes: for K 16 bytes of a key's row (a matrix product does not mind in which order it sums, so the four lanes
 // of a row take the 16-byte pieces as they lie), for V the D/16 bytes at one place of its own eight keys' rows, which it
@@ -856,13 +858,13 @@ __global__ __launch_bounds__(256) void fp8_join_few_kernel(const AttendArgs a) {
 // Many rows per sequence: a workgroup of four waves does 128 rows of one KV head, 32 a wave, over the
 // keys 64 at a time.
 //
-// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 244 us (563 TFLOP/s); 6 chunks of
-// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 751 us (740 TFLOP/s); 5 of up to 700 tokens and
-// 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 39 us.
+// Measured: a prompt of 4096 tokens, 32 query and 8 KV heads of 128, fp16, causal: 137 GFLOP in 250 us (550 TFLOP/s); 6 chunks of
+// up to 900 tokens behind up to 8192, 64 and 8 heads, bf16: 556 GFLOP in 777 us (715 TFLOP/s); 5 of up to 700 tokens and
+// 1500 keys, 16 and 2 heads of 64, fp16, not causal: 9.3 GFLOP in 40 us.
 //
 // Bound by what the matrix products (4 D flops per visible row and key), the softmax beside them (an exp2 and some six other
 // instructions per row and key) and the reads from LDS (a wave's 32 rows need the whole step's K and V) take together: of the
-// second case's time the matrix cores are busy 29 %, the vector units 44 %, LDS 38 %, and two waves to a SIMD, all that
+// second case's time the matrix cores are busy 28 %, the vector units 45 %, LDS 37 %, and two waves to a SIMD, all that
 // registers allow, overlap little of it. So products and softmax are interleaved by halves of a step, and what a step needs from
 // LDS is read half a step ahead. For 64-wide heads it is the length of that chain, 2.3 us a step, also for a wave that has
 // its SIMD to itself. fp16 rows carry P in two halves (see the file's head: P has 11 bits, as much as the output), which makes

@@ -54,7 +54,7 @@ inline AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n
     if (max_len <= 1024) {
       // A workgroup per tile, no second launch: 11.5 us against 16 for a sequence of 500 tokens, 15 against 16 at 1000; at 1500
       // shares are ahead (18.7 against 17.1), and at 4000 by half (35 against 22). Where there are few tiles a head
-      // gets more waves, of more workgroups: 8 sequences of up to 2000 tokens take 22 us, 103 without; but
+      // gets more waves, of more workgroups: 8 sequences of up to 1000 tokens, 8 KV heads, take 14 us, 52 without; 42 of them 21 and 53. But
       // no more workgroups than CUs, each of which holds one (42 short sequences 12.6 us, 19.4 in twice as many).
       auto groups = [&](int32_t per) { return tiles * ((heads + per - 1) / per); };
       while (p.heads_per_group > 1 && groups((p.heads_per_group + 1) / 2) <= 256) p.heads_per_group = (p.heads_per_group + 1) / 2;
@@ -75,9 +75,10 @@ inline AttendPlan plan_fp8_attend(int heads, int group, bool one_each, int64_t n
     p.tiles = tiles_in_all(one_each, group, n_seqs, n_rows, kManyRows);
     // Parts of a tile's keys. The chip holds 512 of these workgroups, two to a CU, so `n` of them take ceil(n / 512) rounds of their
     // steps, and some two steps more to begin and to end (two again where empty workgroups, of tiles that sequences may have
-    // and these do not, take a place first); the parts' sums are written and read again, 115 of them in a step's time. 33 sequences of 40 to 64 rows over 4000 keys, 8 KV heads: 243 us in one part, 184 in three; 300 new
-    // tokens of each of 2 sequences of 3500, 4 KV heads: 52 us in 6 parts, 119 in one and 66 in 12. From 1024 tiles on the rounds
-    // even out by themselves. Parts have four steps at least, and their sums take 140 MB at most.
+    // and these do not, take a place first); the parts' sums are written and read again, 115 of them in a step's time. 33 sequences of
+    // 40 to 64 rows over 4000 keys, 8 KV heads: 243 us in one part, 184 in three; 300 new tokens of each of 2 sequences of 3500, 4
+    // KV heads: 52 us in 6 parts, 119 in one and 66 in 12. From 1024 tiles on the rounds even out by themselves. Parts have
+    // four steps at least, and their sums take 140 MB at most.
     const int64_t tiles_likely = one_each ? p.tiles : all / kManyRows + n_seqs / 2, n = heads * (tiles_likely > n_seqs ? tiles_likely : n_seqs);
     const int64_t steps = steps_of_keys(max_len, kManyKeys);
     p.slots = 1;
