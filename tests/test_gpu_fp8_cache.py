@@ -902,3 +902,42 @@ def test_a_cache_over_tensors_that_want_a_gradient_is_refused(bk, cuda):
             make()
         with torch.no_grad():
             make().close()
+
+
+@pytest.mark.parametrize("wide", [0, 9000])
+@pytest.mark.parametrize("news,G", [([20], 1), ([9], 3), ([140], 2)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_scale_that_is_not_finite_among_scales_far_apart(bk, cuda, value, news, G, wide):
+    """Rows that do not see its page are what they are without it; the others are not finite."""
+    w = World(bk, cuda, [208], news, P=16, H=1, Hq=G, seed=142, wide=wide)
+    w.bytes[1][:, int(w.table[0, 12])] |= 0x08                     # no zero among its bytes: 0 * inf would hide nothing
+    w.scale[1, 1, w.table[0, 1:13:3]] *= 2.0 ** 40
+    w.scale[1, 1, w.table[0, 2]] = 0.0
+    w.push()
+    q = w.randn(G)
+    out, _, tol, _ = _weight_oracle(w, q)
+    w.scale_d[1, 1, int(w.table[0, 12])] = value                   # tokens 192 .. 207
+    got = w.attend(q)
+    w.cache.check()
+    o, first = got[0].cpu().double(), 192 - (208 - news[0])
+    first = max(first, 0)
+    assert ((o[:first] - out[:first]).abs() <= tol[:first]).all() and not o[first:].isfinite().any()
+
+
+def test_scales_far_apart_give_the_same_bits_and_replay_from_a_graph(bk, cuda):
+    for lens, news, G in (([500, 90, 33], [1, 1, 1], 4), ([300, 80], [3, 5], 6), ([700, 300], [200, 140], 2)):
+        w = World(bk, cuda, lens, news, H=2, Hq=2 * G, seed=143, wide=9000 * (G == 4))
+        w.scale[1, 1] *= torch.exp2(torch.randint(-30, 1, w.scale[1, 1].shape, generator=w.g).float())
+        w.push()
+        q = w.randn(2 * G).to(cuda)
+        want = w.cache.attend(1, q, w.table_d, w.lens_d, w.starts_d, return_lse=True)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, lse = w.cache.attend(1, q, w.table_d, w.lens_d, w.starts_d, return_lse=True)
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        _check_weights(w, q.cpu())
