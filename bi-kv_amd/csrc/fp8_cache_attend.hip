@@ -16,9 +16,9 @@
 // the sum of two fp16 numbers. l sums the unrounded p.
 //
 // r: while the V scales of the keys read so far lie within 2^kSpread of each other, the largest one's exponent, the same for all rows of
-// a tile. A row's largest p vs 2^(8 - r) is then 1 at least, whichever of these keys the row sees: a weight p vs keeps its bits
-// down to 2^-14 of the row's largest one, and is off by 2^-25 of that at most below. Once they lie farther apart each
-// row has an r of its own, that of the largest p vs among the keys it does see ("wide" steps, to the end of the tile): a page that a row
+// a tile. A row's largest p vs 2^(8 - r) is then 1 at least, whichever of these keys the row sees: a weight p vs keeps 11 bits
+// down to 2^-14 of the row's largest one, and no weight, of either type, is off by more than 2^-25 of that for want of range. Once they lie farther
+// apart each row has an r of its own, that of the largest p vs among the keys it does see ("wide" steps, to the end of the tile): a page that a row
 // does not see, or hardly attends to, takes no bits from the pages it does. They cost few rows 3 to 8 %, many rows a third.
 #include "fp8_cache_device.h"
 

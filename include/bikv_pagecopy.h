@@ -535,8 +535,8 @@ int bikv_fp8_append(const bikv_fp8_cache* cache, int32_t layer, const bikv_seq_b
  * logarithm of the softmax's sum. A row that sees no key gets out = 0, lse = -inf. Whatever lies in keys a row does
  * not see, NaN included, does not reach it. `workspace`: device memory of bikv_fp8_attend_workspace() bytes (0 = none
  * needed) that belongs to this call until it has run: calls that may overlap take one each. out must not overlap q. A key's weight
- * in a row, its part of the softmax times its page's V scale, is rounded to 11 bits (22 for fp16 tensors); one below 2^-14 of the largest
- * weight among the keys that the row sees is off by up to 2^-25 of that. */
+ * in a row, its part of the softmax times its page's V scale, is rounded to 11 bits (22 for fp16 tensors) or to a multiple of 2^-24 of the
+ * largest weight among the keys that the row sees, whichever is coarser. */
 int64_t bikv_fp8_attend_workspace(const bikv_fp8_cache* cache, const bikv_seq_batch* batch, int32_t q_heads);
 int bikv_fp8_attend(const bikv_fp8_cache* cache, int32_t layer, const bikv_seq_batch* batch,
                     const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t q_heads,
