@@ -12,7 +12,7 @@ scattered from contiguous received buffers into freshly allocated pages, ~10 % o
 shared between requests. One step = one gather launch + one scatter launch over the whole batch.
 Inputs (pool, staging, index arrays) are resident in HBM before the timed region starts.
 
-Prints ONE JSON line. `value` = algorithmic bytes (payload read + payload written) per second over
+Prints ONE JSON line (blocks that would make it longer than 7500 characters go to stderr, `on_stderr` names them). `value` = algorithmic bytes (payload read + payload written) per second over
 the timed steps (400 by default: about two seconds of back-to-back launches); `roofline` prices the
 slower of the two kernels against 8 TB/s with the launch durations measured here with HIP events on
 the launch stream (min / median / p99 per launch are in `kernels`); `cpu_baseline` times the
@@ -229,7 +229,7 @@ def log(msg):
     print(f"[bench] {msg}", file=sys.stderr, flush=True)
 
 
-ALLOC_NOTES = []   # what happened when memory was asked from bikv_device_alloc (reported in the JSON line)
+ALLOC_NOTES = []   # what happened when memory was asked from bikv_device_alloc (reported as `device_alloc`)
 
 
 def spread_empty(bk, nbytes, dev, what):
@@ -1383,9 +1383,22 @@ def run_layout_change(args, bk, dev, blocks=None, sort=False, pool_alloc=None):
     return out
 
 
+LINE_CHARS = 7500   # of the JSON line: records of a run keep some 8000 characters of its output, and a line that is cut is no JSON
+LINE_KEEPS = ("metric", "value", "unit", "n_gpus", "steps", "warmup", "ms_per_step", "higher_is_better", "scaling", "vs_baseline", "dtype", "data",
+              "config", "timed_region_s", "pct_of_hbm_peak", "pages_per_s", "bit_exact", "roofline", "kernels", "cpu_baseline", "summary")
+
+
 def emit(out):
+    """Prints the line. Where it would be too long its longest blocks go to stderr, a line each, and their names stay under `on_stderr`; the
+    summary has their figures."""
     if ALLOC_NOTES:
         out["device_alloc"] = ALLOC_NOTES
+    while len(json.dumps(out)) > LINE_CHARS:
+        size, key = max(((len(json.dumps(v)), k) for k, v in out.items() if k not in LINE_KEEPS and k != "on_stderr"), default=(0, None))
+        if key is None:
+            break
+        log(f"{key}: {json.dumps(out.pop(key))}")
+        out.setdefault("on_stderr", []).append(key)
     if "summary" in out:
         out["summary"] = out.pop("summary")      # keeps it the last key of the line
     print(json.dumps(out), flush=True)

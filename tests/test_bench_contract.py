@@ -65,6 +65,23 @@ def test_summary_block_is_flat_complete_and_last():
     assert list(json.loads(buf.getvalue()).keys())[-1] == "summary"
 
 
+def test_a_long_run_s_line_stays_short_enough_to_be_kept(capsys):
+    """Everything the record is read for stays on the line; the long blocks are whole on stderr."""
+    import bench
+    cells = {"cells": [{"mode": "auto", "passes": list(range(100))} for _ in range(30)]}
+    head = {"metric": "m", "value": 1.5, "unit": "GB/s", "n_gpus": 1, "steps": 20, "warmup": 5, "ms_per_step": 5.0, "higher_is_better": True, "scaling": "weak",
+            "vs_baseline": None, "dtype": "u8", "data": "synthetic", "config": {"workload": "w"}, "roofline": {"bound": "hbm"}}
+    out = dict(head, summary={"value": 1.5}, staging=cells, configs={"a": "b" * 3000}, other_layout={"value": 2.0})
+    bench.emit(out)
+    said = capsys.readouterr()
+    line = json.loads(said.out)
+    assert said.out.count("\n") == 1 and len(said.out) <= 7501 and list(line)[-1] == "summary"
+    assert {k: line[k] for k in head} == head and line["other_layout"] == {"value": 2.0} and line["on_stderr"] == ["staging"]
+    assert json.loads(said.err.split("[bench] staging: ")[1]) == cells
+    bench.emit(dict(head, summary={"value": 1.5}, other_layout={"value": 2.0}))
+    assert "on_stderr" not in json.loads(capsys.readouterr().out)
+
+
 def test_live_traffic_is_computed_from_the_two_counters_and_their_calibration(tmp_path):
     """The figures `roofline.traffic` is made of when the run measures them itself: per-dispatch means of each
     counter for the dominant kernel, each scaled by the same counter's reading for the plain 2 GiB copy. The
